@@ -199,7 +199,7 @@ def _handles(case, s):
         for k in ("logits", "targets", "loss", "dlogits"):
             h[k] = wrap(s[k])
         if case["op"] == "loss_tape":
-            s["stats"] = torch.empty(case["rows"], 2, device="cuda")
+            s["stats"] = torch.empty(case["rows"], 3, device="cuda")
             h["stats"], h["upstream"] = wrap(s["stats"]), wrap(s["upstream"])
     elif case["op"] == "embed":
         s["out"] = torch.empty(case["rows"], case["width"], dtype=s["weight"].dtype, device="cuda")
