@@ -33,7 +33,8 @@
  *    full PCIe bandwidth.  Mixing host and device tensors in one call is an
  *    error.
  *  - dtype: every op implements float32 (RTC_F32).  Other dtypes return
- *    RTC_UNSUPPORTED after the reference's own dtype checks have run.
+ *    RTC_UNSUPPORTED after the reference's own dtype checks have run.  The
+ *    token operators and rtc_adamw_update_multi name the types they take.
  */
 #ifndef RUSTTORCH_CUDA_H
 #define RUSTTORCH_CUDA_H
@@ -53,6 +54,9 @@ extern "C" {
 
 /* dtype codes of CTensorDescriptor.dtype (rusttorch-core/src/ffi/tensor.rs:25) */
 enum { RTC_F32 = 0, RTC_F64 = 1, RTC_I32 = 2, RTC_I64 = 3 };
+/* Types that only the token operators and rtc_adamw_update_multi take (no
+ * reference counterpart); any other call refuses them as unknown codes. */
+enum { RTC_BF16 = 4, RTC_F16 = 5, RTC_F8E4M3 = 6 };
 
 /* rtc_result.code: the TensorError variant (rusttorch-core/src/error.rs:10-67) */
 typedef enum {
@@ -76,7 +80,7 @@ typedef struct {
   const size_t* strides; /* element strides; NULL means C-contiguous */
   size_t ndim;
   size_t numel;          /* must equal the product of shape */
-  int dtype;             /* RTC_F32 ... RTC_I64 */
+  int dtype;             /* RTC_F32 ... RTC_F8E4M3 */
   int device;            /* CUDA device ordinal */
 } rtc_tensor;
 
@@ -105,7 +109,9 @@ rtc_result rtc_set_stream(void* stream);
 void* rtc_get_stream(void);
 /* Waits for the calling thread's stream on its current GPU (rtc_set_device),
  * then reports RTC_BACKEND_ERROR if a kernel on that GPU gave up one of its
- * bounded waits since the last call (its results are then incomplete). */
+ * bounded waits since the last call (its results are then incomplete), or
+ * else RTC_INVALID_ARGUMENT if a token operator met an id or a target outside
+ * its vocabulary since then. */
 rtc_result rtc_synchronize(void);
 /* Failure-path self-test (no reference counterpart): queues a one-thread
  * kernel on the current GPU whose bounded mbarrier wait runs out after 50 ms,
@@ -478,6 +484,88 @@ rtc_result rtc_mean_backward(const rtc_tensor* grad_output, const rtc_tensor* gr
  * for equal element counts, else result[i % m] += grad[i].  Device only. */
 rtc_result rtc_broadcast_add_backward(const rtc_tensor* grad_output, const rtc_tensor* grad_a,
                                       const rtc_tensor* grad_b);
+
+/* ------------------------------------------------------- token operators
+ * No reference counterpart among its ops (its nn::Embedding and the loss over
+ * one-hot targets are host loops).  Device tensors only; asynchronous on the
+ * calling thread's stream; capturable into a CUDA graph.  Ids and targets are
+ * RTC_I32 or RTC_I64; T below is RTC_F32, RTC_BF16 or RTC_F16.  Arithmetic is
+ * in f32 with one rounding to T at the end.  An id or target outside its
+ * vocabulary is never used as an index: the row it would give is NaN (a
+ * gradient skips it) and the next rtc_synchronize on that GPU reports it. */
+
+/* out[i, :] = weight[ids[i], :] * scale: weight [V, D] and out (ids' shape, D)
+ * in T, ids of any shape. */
+rtc_result rtc_embedding(const rtc_tensor* weight, const rtc_tensor* ids, float scale,
+                         const rtc_tensor* out);
+/* The embedding's gradient: grad_weight[v, :] = scale * (the sum of
+ * grad_output[i, :] over the i with ids[i] == v, in f32, in an order that
+ * depends on ids alone), 0 for a v that no id names; with accumulate != 0 that
+ * is added to grad_weight, and rows that no id names are not touched.  Ids
+ * equal to padding_idx (negative: none) contribute nothing.  grad_output (ids' shape, D)
+ * in T; grad_weight [V, D] in f32 or in T; fewer than 2^31 ids. */
+rtc_result rtc_embedding_backward(const rtc_tensor* grad_output, const rtc_tensor* ids,
+                                  float scale, int64_t padding_idx, int accumulate,
+                                  const rtc_tensor* grad_weight);
+
+/* Softmax cross entropy of logits (..., V) in T against token ids.  With
+ * M = max_j x_j and o = the sum of e^(x_j - M) over j != t, a row's loss is
+ * log(o + e^(x_t - M)) - (x_t - M), as log1p(o) where x_t = M.  Rows whose
+ * target is ignore_index have loss and gradient 0.  RTC_REDUCE_MEAN divides
+ * the sum over the other rows by their number (0 if there are none).  `loss`
+ * (f32) has one element, or targets' shape with RTC_REDUCE_NONE.  A row whose
+ * logits are all -inf, or that holds a NaN or +inf, has loss NaN. */
+enum { RTC_REDUCE_NONE = 0, RTC_REDUCE_MEAN = 1, RTC_REDUCE_SUM = 2 };
+/* Forward.  `stats` (f32, targets' shape then 3; may be NULL) receives
+ * M, o + e^(x_t - M) and o for the backward call. */
+rtc_result rtc_softmax_cross_entropy(const rtc_tensor* logits, const rtc_tensor* targets,
+                                     int64_t ignore_index, int reduction, const rtc_tensor* loss,
+                                     const rtc_tensor* stats);
+/* grad_logits (logits' shape and type, may be logits itself) = the forward's
+ * gradient times grad_output (f32, loss's shape, read on the device). */
+rtc_result rtc_softmax_cross_entropy_backward(const rtc_tensor* grad_output,
+                                              const rtc_tensor* logits, const rtc_tensor* targets,
+                                              const rtc_tensor* stats, int64_t ignore_index,
+                                              int reduction, const rtc_tensor* grad_logits);
+/* Loss and gradient in one call, which reads the logits once where a row fits
+ * on chip: loss as the forward's, grad_logits (may be logits itself) = its
+ * gradient times grad_scale. */
+rtc_result rtc_softmax_cross_entropy_grad(const rtc_tensor* logits, const rtc_tensor* targets,
+                                          int64_t ignore_index, int reduction, float grad_scale,
+                                          const rtc_tensor* loss, const rtc_tensor* grad_logits);
+
+/* ops::adamw_update (optimizer.rs:379-440) of n tensors at once, in place,
+ * tensor i of every list on the same GPU (one GPU for the whole call).
+ * params f32; grads f32, RTC_BF16 or RTC_F16; copies (NULL: none) receive each
+ * updated parameter rounded to RTC_BF16 or RTC_F16.
+ *  - m and v f32 (m_scales = v_scales = NULL): with f32 gradients, bit for bit
+ *    what rtc_adamw_update gives for each tensor.
+ *  - m and v RTC_F8E4M3 with scales: moments in 8 bits.  Elements [128b,
+ *    128b + 128) of a tensor share scales[b] (f32, ceil(numel/128) of them), a
+ *    power of two; m's code times its scale is m, v's code times its scale is
+ *    sqrt(v).  Each step decodes, updates in f32
+ *      m' = m*b1 + g*(1-b1), v' = v*b2 + (g*g)*(1-b2), r = sqrt(v'),
+ *      p' = p - (m'/(r*c2 + eps))*(lr/(1-b1^t)) - p*(lr*wd),
+ *      c2 = 1/sqrt(1-b2^t),
+ *    and encodes m' and r with stochastic rounding, so that averages move even
+ *    where one step changes them by less than a code's width: the random bits
+ *    are a function of (seed, i, element) alone.  A non-zero r never becomes 0;
+ *    a moment that is not finite is stored as NaN and leaves its block's scale
+ *    to the others.  rtc_adamw8_pack and _unpack convert from and to f32.
+ * All tensors are checked before anything is launched. */
+rtc_result rtc_adamw_update_multi(const rtc_tensor* params, const rtc_tensor* grads,
+                                  const rtc_tensor* m, const rtc_tensor* v,
+                                  const rtc_tensor* m_scales, const rtc_tensor* v_scales,
+                                  const rtc_tensor* copies, size_t n, double learning_rate,
+                                  double beta1, double beta2, double epsilon, double weight_decay,
+                                  uint64_t timestep, uint64_t seed);
+/* f32 moments m and v (v >= 0) of one tensor to 8 bits, to nearest, and back. */
+rtc_result rtc_adamw8_pack(const rtc_tensor* m, const rtc_tensor* v, const rtc_tensor* m_codes,
+                           const rtc_tensor* m_scales, const rtc_tensor* v_codes,
+                           const rtc_tensor* v_scales);
+rtc_result rtc_adamw8_unpack(const rtc_tensor* m_codes, const rtc_tensor* m_scales,
+                             const rtc_tensor* v_codes, const rtc_tensor* v_scales,
+                             const rtc_tensor* m, const rtc_tensor* v);
 
 /* ------------------------------------------------------------ diagnostics */
 /* Bandwidth probes (no reference counterpart): the read ceiling the

@@ -4,8 +4,8 @@ The Python surface mirrors rusttorch's PyO3 module (rusttorch-py/src/lib.rs):
 the same function names, argument meaning and error behaviour (every failure
 raises ValueError, here the RusttorchError subclass carrying the TensorError
 variant).  The difference is where the data lives: a `Tensor` here is a
-float32 buffer in GPU memory, and every op is one call into
-librusttorch_cuda.so (see include/rusttorch_cuda.h).  Ops are asynchronous on
+buffer in GPU memory (float32, unless a token operator says otherwise), and
+every op is one call into librusttorch_cuda.so (see include/rusttorch_cuda.h).  Ops are asynchronous on
 the calling thread's stream; `to_numpy()` and the scalar reductions wait.
 """
 from __future__ import annotations
@@ -19,7 +19,7 @@ from . import _native
 from ._native import F32, RusttorchError, check, lib
 
 __all__ = [
-    "Tensor", "RusttorchError", "version",
+    "Tensor", "TensorList", "RusttorchError", "version",
     "add", "sub", "mul", "div", "add_scalar", "mul_scalar", "add_mul_scalar",
     "fused_multiply_add", "add_simd", "mul_simd", "relu_simd", "mul_scalar_simd",
     "relu", "leaky_relu", "sigmoid", "tanh", "gelu", "swish", "elu", "selu", "mish",
@@ -29,6 +29,8 @@ __all__ = [
     "add_broadcast", "sub_broadcast", "mul_broadcast", "div_broadcast",
     "nn_adam_step", "nn_sgd_step",
     "synchronize", "set_math_mode", "get_math_mode", "math_mode",
+    "embedding", "embedding_backward", "softmax_cross_entropy", "softmax_cross_entropy_backward",
+    "softmax_cross_entropy_grad", "adamw_update_multi", "adamw8_pack", "adamw8_unpack",
     "sharded_stats", "sharded_add_mul_scalar", "sharded_softmax", "sharded_sum_dim",
     "sharded_mean_dim", "sharded_max_dim", "sharded_adamw_update",
 ]
@@ -73,12 +75,29 @@ def synchronize() -> None:
     check(lib().rtc_synchronize())
 
 
-class Tensor:
-    """A C-contiguous float32 tensor in the memory of one GPU."""
+def _dtype_code(dtype: str) -> int:
+    code = _native.DTYPE_NAMES.get(dtype)
+    if code is None:
+        raise ValueError(f"dtype must be one of {', '.join(_native.DTYPE_NAMES)}, not {dtype!r}")
+    return code
 
-    def __init__(self, shape, device: int = 0, *, ptr: int | None = None, owner=None):
+
+# numpy arrays that Tensor.from_numpy takes, beside float32
+_INDEX_ARRAYS = {np.dtype(np.int32): "int32", np.dtype(np.int64): "int64",
+                 np.dtype(np.float16): "float16"}
+
+
+class Tensor:
+    """A C-contiguous tensor in the memory of one GPU: float32, or for the
+    token operators another `dtype` ("bfloat16", "float16", "float8_e4m3",
+    "int32", "int64")."""
+
+    def __init__(self, shape, device: int = 0, *, ptr: int | None = None, owner=None,
+                 dtype: str = "float32"):
         self._shape = tuple(int(d) for d in shape)
         self.device = int(device)
+        self.dtype = dtype
+        self._code = _dtype_code(dtype)
         self._owned = ptr is None
         self._owner = owner          # keeps a borrowed buffer alive
         if ptr is None:
@@ -86,7 +105,7 @@ class Tensor:
             check(lib().rtc_malloc(self.device, self.nbytes, ctypes.byref(out)))
             ptr = out.value or 0
         self.ptr = int(ptr)
-        self._desc = _native.Desc(self.ptr, self._shape, F32, self.device)
+        self._desc = _native.Desc(self.ptr, self._shape, self._code, self.device)
 
     # ---- construction (rusttorch-py/src/lib.rs:35-61) ---------------------
     @staticmethod
@@ -98,26 +117,41 @@ class Tensor:
         return Tensor.from_numpy(np.ones(list(shape), dtype=np.float32), device)
 
     @staticmethod
-    def empty(shape, device: int = 0) -> "Tensor":
-        return Tensor(shape, device)
+    def empty(shape, device: int = 0, dtype: str = "float32") -> "Tensor":
+        return Tensor(shape, device, dtype=dtype)
 
     @staticmethod
-    def from_numpy(array, device: int = 0) -> "Tensor":
+    def from_numpy(array, device: int = 0, dtype: str | None = None) -> "Tensor":
+        """A copy of the array on the GPU: float32, float16, int32 or int64.
+        With dtype="bfloat16" float32 values are rounded to it (to nearest,
+        ties to even); with dtype="float8_e4m3" uint8 codes are taken as they are."""
         a = np.asarray(array)
-        if a.dtype != np.float32:
-            raise RusttorchError("only float32 arrays are supported", _native.UNSUPPORTED)
+        if dtype == "bfloat16" and a.dtype == np.float32:
+            a = _bf16_bits(a)
+        elif dtype == "float8_e4m3" and a.dtype == np.uint8:
+            pass
+        else:
+            kind = "float32" if a.dtype == np.float32 else _INDEX_ARRAYS.get(a.dtype)
+            if kind is None:
+                raise RusttorchError("only float32 arrays are supported (float16, int32 and int64 "
+                                     "for the token operators)", _native.UNSUPPORTED)
+            if dtype not in (None, kind):
+                raise RusttorchError(f"a {a.dtype} array does not make a {dtype} tensor",
+                                     _native.DTYPE_MISMATCH)
+            dtype = kind
         if not a.flags.c_contiguous:
             raise ValueError("Array must be contiguous")
-        t = Tensor(a.shape, device)
+        t = Tensor(a.shape, device, dtype=dtype)
         if t.nbytes:
             check(lib().rtc_memcpy_h2d(t.device, c_void_p(t.ptr), a.ctypes.data_as(c_void_p),
                                        t.nbytes))
         return t
 
     @staticmethod
-    def from_device_ptr(ptr: int, shape, device: int = 0, owner=None) -> "Tensor":
+    def from_device_ptr(ptr: int, shape, device: int = 0, owner=None,
+                        dtype: str = "float32") -> "Tensor":
         """Borrow an existing device buffer (e.g. a torch tensor's data_ptr())."""
-        return Tensor(shape, device, ptr=ptr, owner=owner)
+        return Tensor(shape, device, ptr=ptr, owner=owner, dtype=dtype)
 
     # ---- metadata (rusttorch-py/src/lib.rs:63-79) -------------------------
     def shape(self) -> list[int]:
@@ -134,16 +168,20 @@ class Tensor:
 
     @property
     def nbytes(self) -> int:
-        return self.numel() * 4
+        return self.numel() * _native.DTYPE_BYTES[self._code]
 
     def __repr__(self) -> str:
-        return f"Tensor(shape={list(self._shape)}, dtype=float32)"
+        return f"Tensor(shape={list(self._shape)}, dtype={self.dtype})"
 
     def to_numpy(self) -> np.ndarray:
-        out = np.empty(self._shape, dtype=np.float32)
+        """The values: bfloat16 as float32, float8_e4m3 as its uint8 codes."""
+        out = np.empty(self._shape, dtype={"bfloat16": np.uint16, "float8_e4m3": np.uint8}.get(
+            self.dtype, self.dtype))
         if self.nbytes:
             check(lib().rtc_memcpy_d2h(self.device, out.ctypes.data_as(c_void_p),
                                        c_void_p(self.ptr), self.nbytes))
+        if self.dtype == "bfloat16":
+            return (out.astype(np.uint32) << 16).view(np.float32)
         return out
 
     @property
@@ -163,6 +201,31 @@ class Tensor:
                 self.ptr = 0
         except Exception:
             pass
+
+
+def _bf16_bits(a: np.ndarray) -> np.ndarray:
+    b = np.ascontiguousarray(a).view(np.uint32)
+    r = ((b + np.uint32(0x7fff) + ((b >> 16) & 1)) >> 16).astype(np.uint16)
+    return np.where(np.isnan(a), np.uint16(0x7fc0), r).reshape(a.shape)
+
+
+class TensorList:
+    """Tensors that are passed to a call together, their descriptors laid out
+    once: an optimizer keeps one for its parameters, gradients and moments.
+    Wherever a function takes a list of tensors it takes one of these."""
+
+    def __init__(self, tensors):
+        self.tensors = tuple(tensors)
+        self._array = _desc_array(self.tensors)
+
+    def __len__(self) -> int:
+        return len(self.tensors)
+
+    def __iter__(self):
+        return iter(self.tensors)
+
+    def __getitem__(self, i):
+        return self.tensors[i]
 
 
 def _like(x: Tensor, shape=None) -> Tensor:
@@ -461,6 +524,130 @@ def binary_cross_entropy_loss(predictions: Tensor, targets: Tensor, epsilon: flo
 
 def cross_entropy_loss(predictions: Tensor, targets: Tensor, epsilon: float = 1e-7) -> float:
     return _loss(lib().rtc_cross_entropy_loss, predictions, targets, float(epsilon))
+
+
+# ---- token operators ---------------------------------------------------------
+# Asynchronous; with `out`, `loss`, `stats` and `grad` given (buffers that a
+# training loop keeps) a call allocates nothing from Python.
+def embedding(weight: Tensor, ids: Tensor, scale: float = 1.0, out: Tensor | None = None) -> Tensor:
+    """weight[ids] * scale: weight [V, D] in float32, bfloat16 or float16, ids
+    of any shape in int32 or int64."""
+    if out is None:
+        width = weight.shape()[1:] if weight.ndim() == 2 else []
+        out = Tensor(ids.shape() + width, weight.device, dtype=weight.dtype)
+    check(lib().rtc_embedding(weight.desc, ids.desc, float(scale), out.desc))
+    return out
+
+
+def embedding_backward(grad_output: Tensor, ids: Tensor, num_embeddings: int, scale: float = 1.0,
+                       padding_idx: int | None = None, accumulate: bool = False,
+                       out: Tensor | None = None) -> Tensor:
+    """The gradient of embedding()'s weight, [num_embeddings, D], in float32
+    unless `out` has grad_output's type.  With accumulate, it is added to
+    `out`, of which only the rows that ids name are touched."""
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs out")
+        width = grad_output.shape()[-1:]
+        out = Tensor([int(num_embeddings)] + width, grad_output.device)
+    elif out.ndim() == 2 and out.shape()[0] != num_embeddings:
+        raise RusttorchError(f"out has {out.shape()[0]} rows, num_embeddings is {num_embeddings}",
+                             _native.SHAPE_MISMATCH)
+    padding = -1 if padding_idx is None else int(padding_idx)
+    if padding_idx is not None and padding < 0:
+        raise RusttorchError("padding_idx must not be negative", _native.INVALID_ARGUMENT)
+    check(lib().rtc_embedding_backward(grad_output.desc, ids.desc, float(scale), padding,
+                                       int(accumulate), out.desc))
+    return out
+
+
+def _reduction(reduction: str) -> int:
+    code = _native.REDUCTIONS.get(reduction)
+    if code is None:
+        raise ValueError(f"reduction must be 'none', 'mean' or 'sum', not {reduction!r}")
+    return code
+
+
+def _loss_out(targets: Tensor, reduction: str, loss: Tensor | None) -> Tensor:
+    if loss is not None:
+        return loss
+    return Tensor(targets.shape() if reduction == "none" else [], targets.device)
+
+
+def softmax_cross_entropy(logits: Tensor, targets: Tensor, ignore_index: int = -100,
+                          reduction: str = "mean", loss: Tensor | None = None,
+                          stats: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """(loss, stats) of logits [..., V] against token ids: loss a float32
+    tensor on the GPU, stats what softmax_cross_entropy_backward needs."""
+    code = _reduction(reduction)
+    loss = _loss_out(targets, reduction, loss)
+    if stats is None:
+        stats = Tensor(targets.shape() + [3], targets.device)
+    check(lib().rtc_softmax_cross_entropy(logits.desc, targets.desc, int(ignore_index), code,
+                                          loss.desc, stats.desc))
+    return loss, stats
+
+
+def softmax_cross_entropy_backward(grad_output: Tensor, logits: Tensor, targets: Tensor,
+                                   stats: Tensor, ignore_index: int = -100,
+                                   reduction: str = "mean", out: Tensor | None = None) -> Tensor:
+    """The gradient of softmax_cross_entropy's logits (out may be logits)."""
+    code = _reduction(reduction)
+    if out is None:
+        out = Tensor(logits.shape(), logits.device, dtype=logits.dtype)
+    check(lib().rtc_softmax_cross_entropy_backward(grad_output.desc, logits.desc, targets.desc,
+                                                   stats.desc, int(ignore_index), code, out.desc))
+    return out
+
+
+def softmax_cross_entropy_grad(logits: Tensor, targets: Tensor, ignore_index: int = -100,
+                               reduction: str = "mean", grad_scale: float = 1.0,
+                               loss: Tensor | None = None,
+                               grad: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """(loss, gradient of the logits times grad_scale) in one pass where a row
+    fits on chip (grad may be logits)."""
+    code = _reduction(reduction)
+    loss = _loss_out(targets, reduction, loss)
+    if grad is None:
+        grad = Tensor(logits.shape(), logits.device, dtype=logits.dtype)
+    check(lib().rtc_softmax_cross_entropy_grad(logits.desc, targets.desc, int(ignore_index), code,
+                                               float(grad_scale), loss.desc, grad.desc))
+    return loss, grad
+
+
+def adamw_update_multi(params, grads, m, v, learning_rate, beta1, beta2, epsilon, weight_decay,
+                       timestep, m_scales=None, v_scales=None, copies=None, seed: int = 0) -> None:
+    """adamw_update of many tensors in place, in few launches (lists of
+    Tensors, or TensorLists).  grads may be float32, bfloat16 or float16.  With
+    float8_e4m3 m and v and their scales (adamw8_pack) the moments are held in
+    8 bits, rounded stochastically from `seed` (another one each step).  copies
+    (bfloat16 or float16) receive the rounded parameters."""
+    lists = [params, grads, m, v, m_scales, v_scales, copies]
+    lists = [t if t is None or isinstance(t, TensorList) else TensorList(t) for t in lists]
+    n = len(lists[0])
+    if any(t is not None and len(t) != n for t in lists):
+        raise ValueError("every list must have as many tensors as params")
+    check(lib().rtc_adamw_update_multi(*(t._array if t is not None else None for t in lists), n,
+                                       learning_rate, beta1, beta2, epsilon, weight_decay,
+                                       int(timestep), int(seed)))
+
+
+def adamw8_pack(m: Tensor, v: Tensor) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(m_codes, m_scales, v_codes, v_scales) of float32 moments, to nearest."""
+    blocks = [-(-m.numel() // _native.MOMENT_BLOCK)]
+    mc, vc = (Tensor(m.shape(), m.device, dtype="float8_e4m3") for _ in range(2))
+    ms, vs = Tensor(blocks, m.device), Tensor(blocks, m.device)
+    check(lib().rtc_adamw8_pack(m.desc, v.desc, mc.desc, ms.desc, vc.desc, vs.desc))
+    return mc, ms, vc, vs
+
+
+def adamw8_unpack(m_codes: Tensor, m_scales: Tensor, v_codes: Tensor,
+                  v_scales: Tensor) -> tuple[Tensor, Tensor]:
+    """The float32 moments that adamw8_pack's or a step's codes stand for."""
+    m, v = _like(m_codes), _like(m_codes)
+    check(lib().rtc_adamw8_unpack(m_codes.desc, m_scales.desc, v_codes.desc, v_scales.desc, m.desc,
+                                  v.desc))
+    return m, v
 
 
 # ---- one process, several GPUs ---------------------------------------------

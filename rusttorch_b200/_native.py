@@ -7,8 +7,8 @@ from __future__ import annotations
 
 import ctypes
 import re
-from ctypes import (POINTER, Structure, c_bool, c_char_p, c_double, c_float, c_int, c_size_t,
-                    c_uint64, c_void_p)
+from ctypes import (POINTER, Structure, c_bool, c_char_p, c_double, c_float, c_int, c_int64,
+                    c_size_t, c_uint64, c_void_p)
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -20,7 +20,14 @@ MATH_TOLERANCE, MATH_EXACT = 0, 1
 # peer-memory exchange (rtc_peer_allreduce_sum_f64)
 IPC_HANDLE_BYTES, PEER_MAX_RANKS = 64, 8
 # dtype codes and status codes (rusttorch_cuda.h)
-F32, F64, I32, I64 = 0, 1, 2, 3
+F32, F64, I32, I64, BF16, F16, F8E4M3 = range(7)
+DTYPE_NAMES = {"float32": F32, "float64": F64, "int32": I32, "int64": I64, "bfloat16": BF16,
+               "float16": F16, "float8_e4m3": F8E4M3}
+DTYPE_BYTES = {F32: 4, F64: 8, I32: 4, I64: 8, BF16: 2, F16: 2, F8E4M3: 1}
+# reductions of the token loss (RTC_REDUCE_*)
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+# elements that share a scale in the 8-bit moments of rtc_adamw_update_multi
+MOMENT_BLOCK = 128
 OK, SHAPE_MISMATCH, DTYPE_MISMATCH, EMPTY_TENSOR, INVALID_DIMENSION, INVALID_ARGUMENT, \
     SIZE_OVERFLOW, UNSUPPORTED, BACKEND_ERROR, BROADCAST_ERROR = range(10)
 STATUS_NAMES = {
@@ -166,6 +173,15 @@ _SIGNATURES = {
     "rtc_sum_backward": (RtcResult, [T, T]),
     "rtc_mean_backward": (RtcResult, [T, T]),
     "rtc_broadcast_add_backward": (RtcResult, [T, T, T]),
+    "rtc_embedding": (RtcResult, [T, T, c_float, T]),
+    "rtc_embedding_backward": (RtcResult, [T, T, c_float, c_int64, c_int, T]),
+    "rtc_softmax_cross_entropy": (RtcResult, [T, T, c_int64, c_int, T, T]),
+    "rtc_softmax_cross_entropy_backward": (RtcResult, [T, T, T, T, c_int64, c_int, T]),
+    "rtc_softmax_cross_entropy_grad": (RtcResult, [T, T, c_int64, c_int, c_float, T, T]),
+    "rtc_adamw_update_multi": (RtcResult, [T, T, T, T, T, T, T, c_size_t, c_double, c_double,
+                                           c_double, c_double, c_double, c_uint64, c_uint64]),
+    "rtc_adamw8_pack": (RtcResult, [T, T, T, T, T, T]),
+    "rtc_adamw8_unpack": (RtcResult, [T, T, T, T, T, T]),
     "rtc_relu_f32": (RtcResult, [c_void_p, c_void_p, c_size_t]),
     "rtc_add_f32": (RtcResult, [c_void_p, c_void_p, c_void_p, c_size_t]),
     "rtc_mul_f32": (RtcResult, [c_void_p, c_void_p, c_void_p, c_size_t]),

@@ -57,10 +57,14 @@ extern "C" rtc_result rtc_synchronize(void) {
   if (e != cudaSuccess) return backend_error("cudaStreamSynchronize", e);
   int device = 0;
   cudaGetDevice(&device);
-  if (take_wait_timeouts(device))
+  const DeviceFlags flags = take_device_flags(device);
+  if (flags.wait_timeout)
     return fail(RTC_BACKEND_ERROR,
                 "a kernel gave up waiting (for a shared-memory tile or another rank; "
                 "2 s limit); results since the last synchronize are incomplete");
+  if (flags.bad_index)
+    return invalid_argument("ids", "a token id or target was outside the vocabulary since the "
+                                   "last synchronize; the rows it gave are NaN");
   return ok();
 }
 
@@ -913,14 +917,32 @@ extern "C" rtc_result rtc_nn_sgd_step(const rtc_tensor* p, const rtc_tensor* g,
 
 // ------------------------------------------------------------- optimizers
 
-// optimizer.rs:242-271, in order.  NaN passes (the comparisons are false).
-static rtc_result adam_hyper_checks(double lr, double b1, double b2, double eps, uint64_t t) {
+rtc_result rt::adam_hyper_checks(double lr, double b1, double b2, double eps, uint64_t t) {
   if (lr <= 0.0) return invalid_argument("learning_rate", "must be positive, got " + rust_f64(lr));
   if (b1 <= 0.0 || b1 >= 1.0) return invalid_argument("beta1", "must be in (0, 1), got " + rust_f64(b1));
   if (b2 <= 0.0 || b2 >= 1.0) return invalid_argument("beta2", "must be in (0, 1), got " + rust_f64(b2));
   if (eps <= 0.0) return invalid_argument("epsilon", "must be positive, got " + rust_f64(eps));
   if (t == 0) return invalid_argument("timestep", "must be >= 1");
   return ok();
+}
+
+AdamCoeffs rt::adam_coeffs(double lr, double b1, double b2, double eps, double wd, uint64_t t,
+                           bool adamw) {
+  const double td = (double)t;
+  const double bc1 = 1.0 - std::pow(b1, td);
+  const double bc2 = 1.0 - std::pow(b2, td);
+  AdamCoeffs c;
+  c.b1 = (float)b1;
+  c.one_minus_b1 = 1.0f - c.b1;
+  c.b2 = (float)b2;
+  c.one_minus_b2 = 1.0f - c.b2;
+  c.bc1 = (float)bc1;
+  c.bc2 = (float)bc2;
+  c.eps = (float)eps;
+  c.lr = (float)lr;
+  c.decay = adamw && wd > 0.0;
+  c.lr_wd = (float)(lr * wd);
+  return c;
 }
 
 static rtc_result adam_common(const rtc_tensor* p, const rtc_tensor* g, const rtc_tensor* m,
@@ -958,21 +980,7 @@ static rtc_result adam_common(const rtc_tensor* p, const rtc_tensor* g, const rt
   TRY(same_device(p, v, po));
   TRY(same_device(p, mo, vo));
   if (p->numel == 0) return ok();
-  // Host-side coefficients, rounded as optimizer.rs:278-309 and :413-418 do.
-  const double td = (double)t;
-  const double bc1 = 1.0 - std::pow(b1, td);
-  const double bc2 = 1.0 - std::pow(b2, td);
-  AdamCoeffs c;
-  c.b1 = (float)b1;
-  c.one_minus_b1 = 1.0f - c.b1;
-  c.b2 = (float)b2;
-  c.one_minus_b2 = 1.0f - c.b2;
-  c.bc1 = (float)bc1;
-  c.bc2 = (float)bc2;
-  c.eps = (float)eps;
-  c.lr = (float)lr;
-  c.decay = adamw && wd > 0.0;
-  c.lr_wd = (float)(lr * wd);
+  const AdamCoeffs c = adam_coeffs(lr, b1, b2, eps, wd, t, adamw);
   if (on_host(p)) {
     const std::vector<size_t> iu{4, 4, 4, 4}, ou{4, 4, 4};
     const std::vector<int> al{0, 2, 3};   // p', m', v' overwrite p, m, v on the device

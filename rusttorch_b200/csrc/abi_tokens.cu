@@ -1,0 +1,480 @@
+// abi_tokens.cu — C-ABI entry points of the token operators (embedding,
+// softmax cross entropy against token ids) and of AdamW over many tensors.
+// Every argument is checked on the host before the CUDA runtime is touched.
+#include "rt_abi_util.h"
+#include "rt_tma.cuh"
+
+#include <algorithm>
+#include <cmath>
+
+using namespace rt;
+
+namespace {
+
+bool store_type(int dtype, StoreType* t) {
+  switch (dtype) {
+    case RTC_F32: *t = kF32; return true;
+    case RTC_BF16: *t = kBF16; return true;
+    case RTC_F16: *t = kF16; return true;
+  }
+  return false;
+}
+
+rtc_result need_float(const rtc_tensor* t, const std::string& what, StoreType* out) {
+  if (!store_type(t->dtype, out))
+    return dtype_mismatch(what, "float32, bfloat16 or float16", dtype_display(t->dtype));
+  return ok();
+}
+
+rtc_result need_ids(const rtc_tensor* t, const std::string& what) {
+  if (t->dtype != RTC_I32 && t->dtype != RTC_I64)
+    return dtype_mismatch(what, "int32 or int64", dtype_display(t->dtype));
+  return ok();
+}
+
+rtc_result need_dtype(const rtc_tensor* t, int dtype, const std::string& what) {
+  if (t->dtype != dtype)
+    return dtype_mismatch(what, dtype_display(dtype), dtype_display(t->dtype));
+  return ok();
+}
+
+rtc_result need_shape(const rtc_tensor* t, const std::vector<size_t>& shape,
+                      const std::string& what) {
+  if (shape_vec(t) != shape) return shape_mismatch_vec(what, shape, shape_vec(t));
+  return ok();
+}
+
+rtc_result one_device(const rtc_tensor* a, const rtc_tensor* b) {
+  if (a->device != b->device)
+    return invalid_argument("device", "all tensors of one call must be on the same device");
+  return ok();
+}
+
+rtc_result apart(const rtc_tensor* out, const rtc_tensor* in, const char* what) {
+  if (overlap(out, in)) return invalid_argument(what, "must not overlap another tensor of the call");
+  return ok();
+}
+
+// `out` may be `in` itself, but not another range over the same bytes.
+rtc_result apart_or_same(const rtc_tensor* out, const rtc_tensor* in, const char* what) {
+  return out->data == in->data ? ok() : apart(out, in, what);
+}
+
+std::vector<size_t> with_last(const rtc_tensor* t, size_t last) {
+  std::vector<size_t> s = shape_vec(t);
+  s.push_back(last);
+  return s;
+}
+
+constexpr size_t kMaxVocab = 0x7fffffff;
+
+// Runs launch(scratch, flag) on the tensors' device.
+template <class F>
+rtc_result on_device(int device, size_t scratch_bytes, const char* what, F launch) {
+  DeviceScope scope(device);
+  if (!scope.ok()) return backend_error("cudaSetDevice", scope.error());
+  int* bad = bad_index_flag(device);
+  if (!bad) return backend_error(what, cudaErrorInvalidValue);
+  if (scratch_bytes == 0) return launched(launch(nullptr, bad), what);
+  Scratch scratch(device, scratch_bytes, thread_stream());
+  if (scratch.error() != cudaSuccess) return backend_error(what, scratch.error());
+  return launched(launch(scratch.get(), bad), what);
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------ embedding
+
+extern "C" rtc_result rtc_embedding(const rtc_tensor* weight, const rtc_tensor* ids, float scale,
+                                    const rtc_tensor* out) {
+  RTC_OP_RANGE();
+  const char* ctx = "embedding";
+  TRY(check_token_desc(weight, "weight"));
+  TRY(check_token_desc(ids, "ids"));
+  TRY(check_token_desc(out, "out"));
+  StoreType type;
+  TRY(need_float(weight, "embedding (weight)", &type));
+  TRY(need_ids(ids, "embedding (ids)"));
+  TRY(need_dtype(out, weight->dtype, "embedding (output)"));
+  if (weight->ndim != 2)
+    return invalid_argument("weight", "must have two dimensions, got " +
+                                          std::to_string(weight->ndim));
+  const size_t vocab = weight->shape[0], width = weight->shape[1];
+  TRY(need_shape(out, with_last(ids, width), "embedding (output)"));
+  if (vocab > kMaxVocab) return invalid_argument("weight", "must have fewer than 2^31 rows");
+  TRY(one_device(weight, ids));
+  TRY(one_device(weight, out));
+  TRY(apart(out, weight, "out"));
+  TRY(apart(out, ids, "out"));
+  if (out->numel == 0) return ok();
+  return on_device(weight->device, 0, ctx, [&](void*, int* bad) {
+    return launch_embedding(type, weight->data, ids->data, ids->dtype == RTC_I64, ids->numel,
+                            vocab, width, scale, out->data, bad, thread_stream());
+  });
+}
+
+extern "C" rtc_result rtc_embedding_backward(const rtc_tensor* grad_output, const rtc_tensor* ids,
+                                             float scale, int64_t padding_idx, int accumulate,
+                                             const rtc_tensor* grad_weight) {
+  RTC_OP_RANGE();
+  const char* ctx = "embedding_backward";
+  TRY(check_token_desc(grad_output, "grad_output"));
+  TRY(check_token_desc(ids, "ids"));
+  TRY(check_token_desc(grad_weight, "grad_weight"));
+  StoreType type, wtype;
+  TRY(need_float(grad_output, "embedding_backward (grad_output)", &type));
+  TRY(need_ids(ids, "embedding_backward (ids)"));
+  TRY(need_float(grad_weight, "embedding_backward (grad_weight)", &wtype));
+  if (wtype != kF32 && wtype != type)
+    return dtype_mismatch("embedding_backward (grad_weight)",
+                          "float32 or " + dtype_display(grad_output->dtype),
+                          dtype_display(grad_weight->dtype));
+  if (grad_weight->ndim != 2)
+    return invalid_argument("grad_weight", "must have two dimensions, got " +
+                                               std::to_string(grad_weight->ndim));
+  const size_t vocab = grad_weight->shape[0], width = grad_weight->shape[1];
+  TRY(need_shape(grad_output, with_last(ids, width), "embedding_backward (grad_output)"));
+  if (vocab > kMaxVocab) return invalid_argument("grad_weight", "must have fewer than 2^31 rows");
+  if (ids->numel > kMaxVocab) return invalid_argument("ids", "must be fewer than 2^31");
+  if (padding_idx >= 0 && (size_t)padding_idx >= vocab)
+    return invalid_argument("padding_idx", "must be below the number of rows (" +
+                                               std::to_string(vocab) + "), got " +
+                                               std::to_string(padding_idx));
+  TRY(one_device(grad_output, ids));
+  TRY(one_device(grad_output, grad_weight));
+  TRY(apart(grad_weight, grad_output, "grad_weight"));
+  TRY(apart(grad_weight, ids, "grad_weight"));
+  if (grad_weight->numel == 0) return ok();
+  return on_device(grad_output->device, embedding_backward_scratch(ids->numel, vocab, width), ctx,
+                   [&](void* scratch, int* bad) {
+                     return launch_embedding_backward(
+                         type, grad_output->data, ids->data, ids->dtype == RTC_I64, ids->numel,
+                         vocab, width, scale, (long long)padding_idx, accumulate != 0,
+                         grad_weight->data, wtype != kF32, scratch, bad, thread_stream());
+                   });
+}
+
+// ------------------------------------------------------ softmax cross entropy
+
+namespace {
+
+rtc_result check_loss(const rtc_tensor* logits, const rtc_tensor* targets, int64_t ignore_index,
+                      int reduction, const std::string& ctx, TokenLoss* a) {
+  TRY(check_token_desc(logits, "logits"));
+  TRY(check_token_desc(targets, "targets"));
+  TRY(need_float(logits, ctx + " (logits)", &a->type));
+  TRY(need_ids(targets, ctx + " (targets)"));
+  if (reduction < RTC_REDUCE_NONE || reduction > RTC_REDUCE_SUM)
+    return invalid_argument("reduction", "must be RTC_REDUCE_NONE, _MEAN or _SUM");
+  if (logits->ndim == 0) return invalid_argument("logits", "must have a last dimension");
+  const size_t vocab = logits->shape[logits->ndim - 1];
+  TRY(need_shape(logits, with_last(targets, vocab), ctx + " (logits vs targets)"));
+  if (vocab == 0) return empty_tensor(ctx);
+  if (vocab > kMaxVocab) return invalid_argument("logits", "must have fewer than 2^31 classes");
+  TRY(one_device(logits, targets));
+  a->logits = logits->data;
+  a->targets = targets->data;
+  a->wide = targets->dtype == RTC_I64;
+  a->rows = targets->numel;
+  a->vocab = vocab;
+  a->ignore = ignore_index;
+  a->reduction = reduction;
+  a->bad = nullptr;
+  return ok();
+}
+
+// One f32 per row, or one in all.
+rtc_result check_row_values(const rtc_tensor* t, const rtc_tensor* logits,
+                            const rtc_tensor* targets, int reduction, const char* name,
+                            const std::string& ctx) {
+  TRY(check_token_desc(t, name));
+  TRY(need_dtype(t, RTC_F32, ctx + " (" + name + ")"));
+  if (reduction == RTC_REDUCE_NONE)
+    TRY(need_shape(t, shape_vec(targets), ctx + " (" + name + ")"));
+  else if (t->numel != 1)
+    return invalid_argument(name, "must have one element, got " + std::to_string(t->numel));
+  return one_device(logits, t);
+}
+
+rtc_result check_grad_logits(const rtc_tensor* logits, const rtc_tensor* targets,
+                             const rtc_tensor* grad, const std::string& ctx) {
+  TRY(check_token_desc(grad, "grad_logits"));
+  TRY(need_dtype(grad, logits->dtype, ctx + " (grad_logits)"));
+  TRY(need_shape(grad, shape_vec(logits), ctx + " (grad_logits)"));
+  TRY(one_device(logits, grad));
+  TRY(apart(grad, targets, "grad_logits"));
+  return apart_or_same(grad, logits, "grad_logits");
+}
+
+rtc_result check_stats(const rtc_tensor* stats, const rtc_tensor* logits,
+                       const rtc_tensor* targets, const std::string& ctx) {
+  TRY(check_token_desc(stats, "stats"));
+  TRY(need_dtype(stats, RTC_F32, ctx + " (stats)"));
+  TRY(need_shape(stats, with_last(targets, 3), ctx + " (stats)"));
+  return one_device(logits, stats);
+}
+
+}  // namespace
+
+extern "C" rtc_result rtc_softmax_cross_entropy(const rtc_tensor* logits,
+                                                const rtc_tensor* targets, int64_t ignore_index,
+                                                int reduction, const rtc_tensor* loss,
+                                                const rtc_tensor* stats) {
+  RTC_OP_RANGE();
+  const char* ctx = "softmax_cross_entropy";
+  TokenLoss a;
+  TRY(check_loss(logits, targets, ignore_index, reduction, ctx, &a));
+  TRY(check_row_values(loss, logits, targets, reduction, "loss", ctx));
+  TRY(apart(loss, logits, "loss"));
+  TRY(apart(loss, targets, "loss"));
+  if (stats) {
+    TRY(check_stats(stats, logits, targets, ctx));
+    TRY(apart(stats, logits, "stats"));
+    TRY(apart(stats, targets, "stats"));
+    TRY(apart(stats, loss, "stats"));
+  }
+  if (a.rows == 0 && reduction == RTC_REDUCE_NONE) return ok();
+  return on_device(logits->device, token_loss_scratch(a), ctx, [&](void* scratch, int* bad) {
+    a.bad = bad;
+    return launch_token_loss(a, f(loss), stats ? f(stats) : nullptr, scratch, thread_stream());
+  });
+}
+
+extern "C" rtc_result rtc_softmax_cross_entropy_backward(
+    const rtc_tensor* grad_output, const rtc_tensor* logits, const rtc_tensor* targets,
+    const rtc_tensor* stats, int64_t ignore_index, int reduction, const rtc_tensor* grad_logits) {
+  RTC_OP_RANGE();
+  const char* ctx = "softmax_cross_entropy_backward";
+  TokenLoss a;
+  TRY(check_loss(logits, targets, ignore_index, reduction, ctx, &a));
+  TRY(check_row_values(grad_output, logits, targets, reduction, "grad_output", ctx));
+  TRY(check_stats(stats, logits, targets, ctx));
+  TRY(check_grad_logits(logits, targets, grad_logits, ctx));
+  TRY(apart(grad_logits, grad_output, "grad_logits"));
+  TRY(apart(grad_logits, stats, "grad_logits"));
+  if (a.rows == 0) return ok();
+  return on_device(logits->device, token_loss_scratch(a), ctx, [&](void* scratch, int* bad) {
+    a.bad = bad;
+    return launch_token_loss_backward(a, cf(grad_output), cf(stats), grad_logits->data, scratch,
+                                      thread_stream());
+  });
+}
+
+extern "C" rtc_result rtc_softmax_cross_entropy_grad(const rtc_tensor* logits,
+                                                     const rtc_tensor* targets,
+                                                     int64_t ignore_index, int reduction,
+                                                     float grad_scale, const rtc_tensor* loss,
+                                                     const rtc_tensor* grad_logits) {
+  RTC_OP_RANGE();
+  const char* ctx = "softmax_cross_entropy_grad";
+  TokenLoss a;
+  TRY(check_loss(logits, targets, ignore_index, reduction, ctx, &a));
+  TRY(check_row_values(loss, logits, targets, reduction, "loss", ctx));
+  TRY(check_grad_logits(logits, targets, grad_logits, ctx));
+  TRY(apart(loss, logits, "loss"));
+  TRY(apart(loss, targets, "loss"));
+  TRY(apart(loss, grad_logits, "loss"));
+  if (a.rows == 0 && reduction == RTC_REDUCE_NONE) return ok();
+  return on_device(logits->device, token_loss_scratch(a), ctx, [&](void* scratch, int* bad) {
+    a.bad = bad;
+    return launch_token_loss_grad(a, grad_scale, f(loss), grad_logits->data, scratch,
+                                  thread_stream());
+  });
+}
+
+// ---------------------------------------------------------- AdamW, many tensors
+
+namespace {
+
+std::string of(const char* list, size_t i) { return std::string(list) + "[" + std::to_string(i) + "]"; }
+
+constexpr size_t kMaxListed = size_t(1) << 20;
+
+// The bytes of one tensor of the lists; `list` names it if it is written.
+struct Range {
+  uintptr_t begin, end;
+  size_t i;
+  const char* list;
+};
+
+void add_range(std::vector<Range>* r, const rtc_tensor* t, size_t i, const char* list) {
+  const uintptr_t b = reinterpret_cast<uintptr_t>(t->data);
+  if (t->numel) r->push_back({b, b + t->numel * dtype_bytes(t->dtype), i, list});
+}
+
+// No written tensor may share bytes with another (the same parameter twice in
+// one call, say): the blocks of both would race.
+rtc_result no_shared_writes(std::vector<Range>* r) {
+  std::sort(r->begin(), r->end(),
+            [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  const Range* written = nullptr;   // of those before: the written one, and the
+  const Range* any = nullptr;       // one at all, that reach furthest
+  for (const Range& x : *r) {
+    const Range* hit = written && written->end > x.begin ? written : nullptr;
+    if (!hit && x.list && any && any->end > x.begin) hit = &x;
+    if (hit)
+      return invalid_argument(of(hit->list, hit->i),
+                              "must not overlap another tensor of the call");
+    if (x.list && (!written || x.end > written->end)) written = &x;
+    if (!any || x.end > any->end) any = &x;
+  }
+  return ok();
+}
+
+rtc_result check_moments(const rtc_tensor* p, const rtc_tensor* codes, const rtc_tensor* scales,
+                         const std::string& name, const std::string& scale_name) {
+  TRY(need_dtype(codes, RTC_F8E4M3, name));
+  TRY(check_token_desc(scales, scale_name.c_str()));
+  TRY(need_dtype(scales, RTC_F32, scale_name));
+  const size_t blocks = (p->numel + kMomentBlock - 1) / kMomentBlock;
+  if (scales->numel != blocks)
+    return invalid_argument(scale_name, "must have one element per " +
+                                            std::to_string(kMomentBlock) + " (" +
+                                            std::to_string(blocks) + "), got " +
+                                            std::to_string(scales->numel));
+  return one_device(p, scales);
+}
+
+}  // namespace
+
+extern "C" rtc_result rtc_adamw_update_multi(
+    const rtc_tensor* params, const rtc_tensor* grads, const rtc_tensor* m, const rtc_tensor* v,
+    const rtc_tensor* m_scales, const rtc_tensor* v_scales, const rtc_tensor* copies, size_t n,
+    double learning_rate, double beta1, double beta2, double epsilon, double weight_decay,
+    uint64_t timestep, uint64_t seed) {
+  RTC_OP_RANGE();
+  if (n == 0) return ok();
+  if (!params) return invalid_argument("params", "must not be null");
+  if (!grads) return invalid_argument("grads", "must not be null");
+  if (!m) return invalid_argument("m", "must not be null");
+  if (!v) return invalid_argument("v", "must not be null");
+  if (!m_scales != !v_scales)
+    return invalid_argument("v_scales", "m_scales and v_scales must both be given or both be null");
+  const bool eight = m_scales != nullptr;
+  if (n > kMaxListed)
+    return invalid_argument("n", "must be at most " + std::to_string(kMaxListed) + " tensors");
+  if (weight_decay < 0.0)
+    return invalid_argument("weight_decay", "must be non-negative, got " + rust_f64(weight_decay));
+  std::vector<AdamTensor> list(n);
+  std::vector<Range> ranges;
+  ranges.reserve(7 * n);
+  for (size_t i = 0; i < n; i++) {
+    const rtc_tensor* p = &params[i];
+    TRY(check_token_desc(p, of("params", i).c_str()));
+    TRY(check_token_desc(&grads[i], of("grads", i).c_str()));
+    TRY(check_token_desc(&m[i], of("m", i).c_str()));
+    TRY(check_token_desc(&v[i], of("v", i).c_str()));
+    AdamTensor& t = list[i];
+    TRY(need_dtype(p, RTC_F32, of("params", i)));
+    TRY(need_float(&grads[i], of("grads", i), &t.gtype));
+    if (!same_shape(p, &grads[i])) return shape_mismatch(of("grads", i), p, &grads[i]);
+    if (!same_shape(p, &m[i])) return shape_mismatch(of("m", i), p, &m[i]);
+    if (!same_shape(p, &v[i])) return shape_mismatch(of("v", i), p, &v[i]);
+    TRY(one_device(&params[0], p));
+    TRY(one_device(p, &grads[i]));
+    TRY(one_device(p, &m[i]));
+    TRY(one_device(p, &v[i]));
+    t.ms = t.vs = nullptr;
+    if (eight) {
+      TRY(check_moments(p, &m[i], &m_scales[i], of("m", i), of("m_scales", i)));
+      TRY(check_moments(p, &v[i], &v_scales[i], of("v", i), of("v_scales", i)));
+      t.ms = f(&m_scales[i]);
+      t.vs = f(&v_scales[i]);
+    } else {
+      TRY(need_dtype(&m[i], RTC_F32, of("m", i)));
+      TRY(need_dtype(&v[i], RTC_F32, of("v", i)));
+    }
+    t.copy = nullptr;
+    t.ctype = kBF16;
+    if (copies) {
+      TRY(check_token_desc(&copies[i], of("copies", i).c_str()));
+      if (copies[i].dtype != RTC_BF16 && copies[i].dtype != RTC_F16)
+        return dtype_mismatch(of("copies", i), "bfloat16 or float16",
+                              dtype_display(copies[i].dtype));
+      if (!same_shape(p, &copies[i])) return shape_mismatch(of("copies", i), p, &copies[i]);
+      TRY(one_device(p, &copies[i]));
+      store_type(copies[i].dtype, &t.ctype);
+      t.copy = copies[i].data;
+    }
+    t.p = f(p);
+    t.g = grads[i].data;
+    t.m = m[i].data;
+    t.v = v[i].data;
+    t.n = p->numel;
+    add_range(&ranges, p, i, "params");
+    add_range(&ranges, &grads[i], i, nullptr);
+    add_range(&ranges, &m[i], i, "m");
+    add_range(&ranges, &v[i], i, "v");
+    if (eight) {
+      add_range(&ranges, &m_scales[i], i, "m_scales");
+      add_range(&ranges, &v_scales[i], i, "v_scales");
+    }
+    if (copies) add_range(&ranges, &copies[i], i, "copies");
+  }
+  TRY(no_shared_writes(&ranges));
+  TRY(adam_hyper_checks(learning_rate, beta1, beta2, epsilon, timestep));
+  return on_device(params[0].device, 0, "adamw_update_multi", [&](void*, int*) {
+    const AdamCoeffs c =
+        adam_coeffs(learning_rate, beta1, beta2, epsilon, weight_decay, timestep, true);
+    if (!eight) return launch_adam_multi(list.data(), n, c, thread_stream());
+    Adam8Coeffs c8;
+    c8.b1 = c.b1;
+    c8.one_minus_b1 = c.one_minus_b1;
+    c8.b2 = c.b2;
+    c8.one_minus_b2 = c.one_minus_b2;
+    c8.c2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)timestep)));
+    c8.eps = c.eps;
+    c8.step = (float)(learning_rate / (1.0 - std::pow(beta1, (double)timestep)));
+    c8.lr_wd = c.lr_wd;
+    c8.decay = c.decay;
+    return launch_adam8_multi(list.data(), n, c8, seed, thread_stream());
+  });
+}
+
+namespace {
+rtc_result check_packed(const rtc_tensor* m, const rtc_tensor* v, const rtc_tensor* mc,
+                        const rtc_tensor* ms, const rtc_tensor* vc, const rtc_tensor* vs) {
+  TRY(check_token_desc(m, "m"));
+  TRY(check_token_desc(v, "v"));
+  TRY(check_token_desc(mc, "m_codes"));
+  TRY(check_token_desc(vc, "v_codes"));
+  TRY(need_dtype(m, RTC_F32, "m"));
+  TRY(need_dtype(v, RTC_F32, "v"));
+  if (!same_shape(m, v)) return shape_mismatch("v", m, v);
+  if (!same_shape(m, mc)) return shape_mismatch("m_codes", m, mc);
+  if (!same_shape(m, vc)) return shape_mismatch("v_codes", m, vc);
+  TRY(one_device(m, v));
+  TRY(one_device(m, mc));
+  TRY(one_device(m, vc));
+  TRY(check_moments(m, mc, ms, "m_codes", "m_scales"));
+  TRY(check_moments(m, vc, vs, "v_codes", "v_scales"));
+  const rtc_tensor* all[6] = {m, v, mc, ms, vc, vs};
+  for (int i = 0; i < 6; i++)
+    for (int j = 0; j < i; j++) TRY(apart(all[i], all[j], "tensors"));
+  return ok();
+}
+}  // namespace
+
+extern "C" rtc_result rtc_adamw8_pack(const rtc_tensor* m, const rtc_tensor* v,
+                                      const rtc_tensor* m_codes, const rtc_tensor* m_scales,
+                                      const rtc_tensor* v_codes, const rtc_tensor* v_scales) {
+  RTC_OP_RANGE();
+  TRY(check_packed(m, v, m_codes, m_scales, v_codes, v_scales));
+  if (m->numel == 0) return ok();
+  return on_device(m->device, 0, "adamw8_pack", [&](void*, int*) {
+    return launch_adam8_pack(cf(m), cf(v), m_codes->data, f(m_scales), v_codes->data, f(v_scales),
+                             m->numel, thread_stream());
+  });
+}
+
+extern "C" rtc_result rtc_adamw8_unpack(const rtc_tensor* m_codes, const rtc_tensor* m_scales,
+                                        const rtc_tensor* v_codes, const rtc_tensor* v_scales,
+                                        const rtc_tensor* m, const rtc_tensor* v) {
+  RTC_OP_RANGE();
+  TRY(check_packed(m, v, m_codes, m_scales, v_codes, v_scales));
+  if (m->numel == 0) return ok();
+  return on_device(m->device, 0, "adamw8_unpack", [&](void*, int*) {
+    return launch_adam8_unpack(m_codes->data, cf(m_scales), v_codes->data, cf(v_scales), f(m),
+                               f(v), m->numel, thread_stream());
+  });
+}

@@ -10,6 +10,7 @@
 // Little's law asks for at HBM3e latency.  Loads and stores use the streaming
 // cache hint (.cs): every byte is touched once.  Pointers that are not all
 // 16-byte aligned take a scalar grid-stride kernel instead (same results).
+#include "rt_adam.cuh"
 #include "rt_internal.h"
 #include "rt_map.cuh"
 #include "rt_ops.cuh"
@@ -121,21 +122,6 @@ cudaError_t launch_fma(const float* a, const float* b, const float* c, float* ou
 // ----------------------------------------------------------------- optimizers
 
 namespace {
-
-// One Adam/AdamW element, in the order of optimizer.rs:293-309 and :413-421.
-__device__ __forceinline__ void adam1(const AdamCoeffs& c, float p, float g, float m, float v,
-                                      float& po, float& mo, float& vo) {
-  const float nm = fadd(fmul(m, c.b1), fmul(g, c.one_minus_b1));
-  const float nv = fadd(fmul(v, c.b2), fmul(fmul(g, g), c.one_minus_b2));
-  const float mh = fdiv(nm, c.bc1);
-  const float vh = fdiv(nv, c.bc2);
-  const float den = fadd(fsqrt(vh), c.eps);
-  float np = fsub(p, fmul(fdiv(mh, den), c.lr));
-  if (c.decay) np = fsub(np, fmul(p, c.lr_wd));
-  po = np;
-  mo = nm;
-  vo = nv;
-}
 
 template <int U>
 __global__ void __launch_bounds__(kThreads)

@@ -120,6 +120,9 @@ std::string dtype_debug(int dtype) {
     case RTC_F64: return "Float64";
     case RTC_I32: return "Int32";
     case RTC_I64: return "Int64";
+    case RTC_BF16: return "BFloat16";
+    case RTC_F16: return "Float16";
+    case RTC_F8E4M3: return "Float8E4M3";
   }
   return "Unknown(" + std::to_string(dtype) + ")";
 }
@@ -130,15 +133,18 @@ std::string dtype_display(int dtype) {
     case RTC_F64: return "float64";
     case RTC_I32: return "int32";
     case RTC_I64: return "int64";
+    case RTC_BF16: return "bfloat16";
+    case RTC_F16: return "float16";
+    case RTC_F8E4M3: return "float8_e4m3";
   }
   return "unknown(" + std::to_string(dtype) + ")";
 }
 
 // --------------------------------------------------------------- descriptors
 
-rtc_result check_desc(const rtc_tensor* t, const char* name) {
+static rtc_result check_desc_to(const rtc_tensor* t, const char* name, int last_dtype) {
   if (!t) return invalid_argument(name, "tensor descriptor must not be null");
-  if (t->dtype < RTC_F32 || t->dtype > RTC_I64)
+  if (t->dtype < RTC_F32 || t->dtype > last_dtype)
     return invalid_argument("dtype", "Unknown dtype code: " + std::to_string(t->dtype));
   if (t->ndim > 0 && !t->shape) return invalid_argument(name, "shape must not be null");
   size_t prod = 1;
@@ -164,6 +170,38 @@ rtc_result check_desc(const rtc_tensor* t, const char* name) {
   }
   if (t->numel > 0 && !t->data) return invalid_argument(name, "data must not be null");
   return ok();
+}
+
+rtc_result check_desc(const rtc_tensor* t, const char* name) {
+  return check_desc_to(t, name, RTC_I64);
+}
+
+rtc_result check_token_desc(const rtc_tensor* t, const char* name) {
+  TRY(check_desc_to(t, name, RTC_F8E4M3));
+  if (t->device == RTC_HOST_MEMORY)
+    return invalid_argument("device", std::string(name) + " must be a device tensor");
+  if (t->device < 0) return invalid_argument("device", "invalid device ordinal");
+  if (t->numel > 0 && reinterpret_cast<uintptr_t>(t->data) % dtype_bytes(t->dtype) != 0)
+    return invalid_argument(name, "data must be aligned to its element type");
+  return ok();
+}
+
+size_t dtype_bytes(int dtype) {
+  switch (dtype) {
+    case RTC_F64:
+    case RTC_I64: return 8;
+    case RTC_BF16:
+    case RTC_F16: return 2;
+    case RTC_F8E4M3: return 1;
+  }
+  return 4;
+}
+
+bool overlap(const rtc_tensor* a, const rtc_tensor* b) {
+  if (a->device != b->device) return false;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a->data), y = reinterpret_cast<uintptr_t>(b->data);
+  const size_t nx = a->numel * dtype_bytes(a->dtype), ny = b->numel * dtype_bytes(b->dtype);
+  return nx && ny && x < y + ny && y < x + nx;
 }
 
 bool is_float(int dtype) { return dtype == RTC_F32 || dtype == RTC_F64; }

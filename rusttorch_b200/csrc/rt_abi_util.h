@@ -64,6 +64,12 @@ struct OpRange {
 
 // ---- descriptors ------------------------------------------------------------
 rtc_result check_desc(const rtc_tensor* t, const char* name);   // structural sanity
+// The same for the token operators, which take the types up to RTC_F8E4M3 and
+// device memory only.
+rtc_result check_token_desc(const rtc_tensor* t, const char* name);
+size_t dtype_bytes(int dtype);
+// Whether the two tensors' bytes overlap.
+bool overlap(const rtc_tensor* a, const rtc_tensor* b);
 bool is_float(int dtype);
 bool same_shape(const rtc_tensor* a, const rtc_tensor* b);
 std::vector<size_t> shape_vec(const rtc_tensor* t);
@@ -99,6 +105,36 @@ void keep_pool_memory(int device);
 void release_library_state();
 // Destroys the per-device streams of the sharded entry points (abi_sharded.cu).
 void release_sharded_streams();
+
+// Scratch of one call from the stream-ordered pool, on the current device;
+// freed behind the work that the call queued.
+class Scratch {
+ public:
+  Scratch(int device, size_t bytes, cudaStream_t s) : s_(s) {
+    keep_pool_memory(device);
+    err_ = cudaMallocAsync(&p_, bytes, s);
+    if (err_ != cudaSuccess) p_ = nullptr;
+  }
+  ~Scratch() {
+    if (p_) cudaFreeAsync(p_, s_);
+  }
+  Scratch(const Scratch&) = delete;
+  Scratch& operator=(const Scratch&) = delete;
+  void* get() const { return p_; }
+  cudaError_t error() const { return err_; }
+
+ private:
+  cudaStream_t s_;
+  void* p_ = nullptr;
+  cudaError_t err_ = cudaSuccess;
+};
+
+// ---- optimizer checks shared by the one- and many-tensor entry points -------
+// optimizer.rs:242-271, in order.  NaN passes (the comparisons are false).
+rtc_result adam_hyper_checks(double lr, double b1, double b2, double eps, uint64_t t);
+// Coefficients rounded as optimizer.rs:278-309 and :413-418 do.
+AdamCoeffs adam_coeffs(double lr, double b1, double b2, double eps, double wd, uint64_t t,
+                       bool adamw);
 
 // ---- exact global statistics ------------------------------------------------
 // Sum (f64) and the reference's max/min fold results of x[0..n), n > 0.

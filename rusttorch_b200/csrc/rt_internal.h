@@ -190,6 +190,77 @@ size_t ordered_sum_scratch_bytes(size_t n, int chains);
 cudaError_t launch_softmax(const float* x, size_t outer, size_t len, size_t inner,
                            bool last_axis, float* out, cudaStream_t s);
 
+// ------------------------------------------------------------ token operators
+// A storage type of the token operators, as a launcher's argument.
+enum StoreType { kF32, kBF16, kF16 };
+size_t store_bytes(StoreType t);
+
+// out[i, :] = weight[ids[i], :] * scale (embedding.cu).  ids: n of them, int64
+// when `wide`.  `bad` is the device flag raised for an id outside [0, vocab).
+cudaError_t launch_embedding(StoreType t, const void* weight, const void* ids, bool wide,
+                             size_t n, size_t vocab, size_t width, float scale, void* out,
+                             int* bad, cudaStream_t s);
+// grad_weight (f32, or the gradient's type when `narrow`) from grad_output.
+// padding < 0: none.  `scratch`: embedding_backward_scratch bytes, 256-byte
+// aligned.
+size_t embedding_backward_scratch(size_t n, size_t vocab, size_t width);
+cudaError_t launch_embedding_backward(StoreType t, const void* grad_output, const void* ids,
+                                      bool wide, size_t n, size_t vocab, size_t width,
+                                      float scale, long long padding, bool accumulate,
+                                      void* grad_weight, bool narrow, void* scratch, int* bad,
+                                      cudaStream_t s);
+
+// Softmax cross entropy against token ids (token_loss.cu).
+struct TokenLoss {
+  StoreType type;
+  const void* logits;    // [rows, vocab]
+  const void* targets;   // [rows]
+  bool wide;             // targets are int64
+  size_t rows, vocab;
+  long long ignore;
+  int reduction;         // RTC_REDUCE_*
+  int* bad;
+};
+// Scratch of the calls below, 256-byte aligned.
+size_t token_loss_scratch(const TokenLoss& a);
+// loss and, unless null, stats [rows, 3].
+cudaError_t launch_token_loss(const TokenLoss& a, float* loss, float* stats, void* scratch,
+                              cudaStream_t s);
+// grad from stats; `upstream` has 1 element, or `rows` with RTC_REDUCE_NONE.
+cudaError_t launch_token_loss_backward(const TokenLoss& a, const float* upstream,
+                                       const float* stats, void* grad, void* scratch,
+                                       cudaStream_t s);
+// Both; the gradient is multiplied by grad_scale.
+cudaError_t launch_token_loss_grad(const TokenLoss& a, float grad_scale, float* loss, void* grad,
+                                   void* scratch, cudaStream_t s);
+
+// ------------------------------------------------------------ many tensors
+// One tensor of a many-tensor AdamW step (adam_multi.cu).
+struct AdamTensor {
+  float* p;
+  const void* g;
+  void *m, *v;           // f32, or e4m3 codes
+  float *ms, *vs;        // scales of the 8-bit moments, else null
+  void* copy;            // null: none
+  unsigned long long n;
+  StoreType gtype, ctype;
+};
+// Elements that share a scale in the 8-bit moments.
+constexpr int kMomentBlock = 128;
+// Coefficients of a step with 8-bit moments.
+struct Adam8Coeffs {
+  float b1, one_minus_b1, b2, one_minus_b2, c2, eps, step;
+  float lr_wd;
+  int decay;
+};
+cudaError_t launch_adam_multi(const AdamTensor* t, size_t n, const AdamCoeffs& c, cudaStream_t s);
+cudaError_t launch_adam8_multi(const AdamTensor* t, size_t n, const Adam8Coeffs& c, uint64_t seed,
+                               cudaStream_t s);
+cudaError_t launch_adam8_pack(const float* m, const float* v, void* mc, float* ms, void* vc,
+                              float* vs, size_t n, cudaStream_t s);
+cudaError_t launch_adam8_unpack(const void* mc, const float* ms, const void* vc, const float* vs,
+                                float* m, float* v, size_t n, cudaStream_t s);
+
 // ------------------------------------------------------------------ generator
 cudaError_t launch_fill(float* out, size_t n, uint64_t seed, uint64_t offset, float a, float b,
                         int normal, cudaStream_t s);

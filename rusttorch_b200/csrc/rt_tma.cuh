@@ -111,9 +111,17 @@ bool encode_tensor_map_f32(CUtensorMap* tm, const void* base, int rank, const ui
 // address is looked up once per device and kept, so the library must not be
 // used on a device after that device has been reset.
 int* wait_timeout_flag(int device);
-// Host: nonzero if a kernel on `device` gave up a bounded wait since the
-// last call (the flag is cleared).  Synchronises the device's work first.
-int take_wait_timeouts(int device);
+// Host: the flag a kernel sets (to 1) when a token id or target lies outside
+// its vocabulary; as wait_timeout_flag.
+int* bad_index_flag(int device);
+// Host: whether a kernel on `device` gave up a bounded wait, or met an index
+// outside its vocabulary, since the last call (the flags are cleared).
+// Synchronises the device's work first.
+struct DeviceFlags {
+  bool wait_timeout = false;
+  bool bad_index = false;
+};
+DeviceFlags take_device_flags(int device);
 // Host: launches a one-thread kernel whose bounded wait runs out (50 ms), to
 // exercise the timeout path: the next rtc_synchronize reports it.
 cudaError_t launch_bounded_wait_probe(int device, cudaStream_t s);

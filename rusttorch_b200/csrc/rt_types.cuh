@@ -1,0 +1,56 @@
+// rt_types.cuh — the storage types of the token operators: conversions to and
+// from f32, and 16-byte groups of elements.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+namespace rt {
+
+using bf16 = __nv_bfloat16;
+using f16 = __half;
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(bf16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(f16 x) { return __half2float(x); }
+
+// Rounded to nearest, ties to even (f16: to infinity beyond 65504).
+template <class T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ bf16 from_f32<bf16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ f16 from_f32<f16>(float x) { return __float2half_rn(x); }
+
+// 16 bytes of elements, moved by one load or store.
+template <class T>
+struct alignas(16) Pack {
+  static constexpr int N = 16 / sizeof(T);
+  T x[N];
+};
+
+// Loads and stores that each touch their bytes once (evict-first).
+template <class T>
+__device__ __forceinline__ Pack<T> ld_pack(const T* p) {
+  const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
+  return *reinterpret_cast<const Pack<T>*>(&v);
+}
+template <class T>
+__device__ __forceinline__ void st_pack(T* p, const Pack<T>& v) {
+  __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&v));
+}
+
+// Ids and targets: 32- or 64-bit integers, read as 64.
+struct IndexArray {
+  const void* p;
+  bool wide;   // int64
+  __device__ __forceinline__ long long operator[](size_t i) const {
+    return wide ? static_cast<const long long*>(p)[i]
+                : (long long)static_cast<const int*>(p)[i];
+  }
+};
+
+}  // namespace rt

@@ -12,7 +12,9 @@
 namespace rt {
 namespace {
 
-__device__ int g_wait_timeouts;
+// [0]: a kernel gave up a bounded wait; [1]: a token id or target was outside
+// its vocabulary.  One array, so that one copy reads both.
+__device__ int g_flags[2];
 
 std::mutex g_mu;
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
@@ -58,21 +60,26 @@ int* wait_timeout_flag(int device) {
   if ((size_t)device >= g_flag.size()) g_flag.resize(device + 1, nullptr);
   if (!g_flag[device]) {
     void* p = nullptr;
-    if (cudaGetSymbolAddress(&p, g_wait_timeouts) != cudaSuccess) return nullptr;
+    if (cudaGetSymbolAddress(&p, g_flags) != cudaSuccess) return nullptr;
     g_flag[device] = static_cast<int*>(p);
   }
   return g_flag[device];
 }
 
-int take_wait_timeouts(int device) {
-  if (!wait_timeout_flag(device)) return 0;
-  int v = 0;
-  if (cudaMemcpyFromSymbol(&v, g_wait_timeouts, sizeof(int)) != cudaSuccess) return 0;
-  if (v) {
-    const int zero = 0;
-    cudaMemcpyToSymbol(g_wait_timeouts, &zero, sizeof(int));
+int* bad_index_flag(int device) {
+  int* p = wait_timeout_flag(device);
+  return p ? p + 1 : nullptr;
+}
+
+DeviceFlags take_device_flags(int device) {
+  if (!wait_timeout_flag(device)) return {};
+  int v[2] = {0, 0};
+  if (cudaMemcpyFromSymbol(v, g_flags, sizeof v) != cudaSuccess) return {};
+  if (v[0] || v[1]) {
+    const int zero[2] = {0, 0};
+    cudaMemcpyToSymbol(g_flags, zero, sizeof zero);
   }
-  return v;
+  return {v[0] != 0, v[1] != 0};
 }
 
 namespace {
