@@ -1,7 +1,24 @@
 // embedding.cu — rows of a table by token id, and the table's gradient.
+//
+// Forward: out[i, :] = T(scale * weight[ids[i], :]), one f32 product and one
+// rounding per element.  A group of threads walks a row, 16 bytes a thread.
+//
+// Gradient: grad_weight[v, :] (+)= scale * sum over {i : ids[i] = v} of
+// grad_output[i, :].  The sums of a row are wherever its tokens are, so:
+//  1. sort_ids_kernel sorts the positions by id (stable radix sort) in one
+//     cluster of thread blocks, and marks which ids occur;
+//  2. segment_kernel cuts the sorted list into pieces of equal length, so
+//     that a frequent id costs no block more than a rare one; a group sums its
+//     piece's rows in order, writes each id's sum that begins and ends in the
+//     piece, and leaves partial sums of those that cross its ends; in the same
+//     launch other blocks write the zeros of the ids that do not occur;
+//  3. join_kernel adds up the partial sums.
+// No floating-point atomics: the order of every sum follows from ids alone.
 #include "rt_internal.h"
 #include "rt_libm.cuh"
 #include "rt_types.cuh"
+
+#include <cooperative_groups.h>
 
 #include <algorithm>
 
@@ -11,57 +28,595 @@ size_t store_bytes(StoreType t) { return t == kF32 ? 4 : 2; }
 
 namespace {
 
+namespace cg = cooperative_groups;
+
+// ---- rows, 16 bytes to a thread ---------------------------------------------
+// A group of G threads covers G * 16 bytes of a row: each thread N / VW chunks
+// of VW elements, G chunks apart.  VW is the widest access that every row's
+// start allows (16 bytes down to one element).
+template <class T, int VW>
+struct alignas(VW * sizeof(T)) Chunk {
+  T x[VW];
+};
+
 template <class T>
-__global__ void __launch_bounds__(kThreads)
-embedding_kernel(const T* w, IndexArray ids, size_t n, long long vocab, size_t width, float scale,
-                 T* out, int* bad) {
-  for (size_t i = blockIdx.x; i < n; i += gridDim.x) {
-    const long long id = ids[i];
-    const bool good = id >= 0 && id < vocab;
-    if (!good && threadIdx.x == 0) atomicExch(bad, 1);
-    for (size_t c = threadIdx.x; c < width; c += kThreads)
-      out[i * width + c] =
-          from_f32<T>(good ? fmul(to_f32(w[(size_t)id * width + c]), scale) : u2f(0x7fc00000u));
+struct Row {
+  static constexpr int N = 16 / sizeof(T);
+  T x[N];
+};
+
+template <int VW, bool ONCE, class T>
+__device__ __forceinline__ void load_row(const T* row, size_t first, unsigned G, size_t width,
+                                         Row<T>& r) {
+  constexpr int N = Row<T>::N;
+#pragma unroll
+  for (int k = 0; k < N / VW; k++) {
+    const size_t c = first + (size_t)k * G * VW;
+    if (c < width) {
+      const T* p = row + c;
+      if constexpr (VW * sizeof(T) == 16) {
+        const uint4* q = reinterpret_cast<const uint4*>(p);
+        const uint4 v = ONCE ? __ldcs(q) : __ldg(q);
+        *reinterpret_cast<uint4*>(&r.x[k * VW]) = v;
+      } else {
+        const auto v = *reinterpret_cast<const Chunk<T, VW>*>(p);
+#pragma unroll
+        for (int e = 0; e < VW; e++) r.x[k * VW + e] = v.x[e];
+      }
+    }
   }
 }
 
-// One block per table row: it looks through all ids for its own.
-template <class T, class G>
-__global__ void __launch_bounds__(kThreads)
-embedding_backward_kernel(const T* g, IndexArray ids, size_t n, long long vocab, size_t width,
-                          float scale, long long padding, bool accumulate, G* gw, int* bad) {
-  __shared__ int hits[kThreads];
-  __shared__ int count;
-  const size_t col = (size_t)blockIdx.y * kThreads + threadIdx.x;
-  for (long long v = blockIdx.x; v < vocab; v += gridDim.x) {
-    float acc = 0.0f;
-    bool any = false;
-    for (size_t base = 0; base < n; base += kThreads) {
-      const size_t i = base + threadIdx.x;
-      const long long id = i < n ? ids[i] : -1;
-      if (i < n && (id < 0 || id >= vocab)) atomicExch(bad, 1);
-      hits[threadIdx.x] = id == v && v != padding;
-      const int found = __syncthreads_count(hits[threadIdx.x]);
-      if (found) {
-        any = true;
-        if (threadIdx.x == 0) {
-          count = 0;
-          for (int k = 0; k < kThreads; k++)
-            if (hits[k]) hits[count++] = k;
-        }
-        __syncthreads();
-        if (col < width)
-          for (int k = 0; k < found; k++)
-            acc = fadd(acc, to_f32(g[(base + hits[k]) * width + col]));
+// Stores values laid out as load_row<VW> gave them.
+template <int VW, class G_, int N>
+__device__ __forceinline__ void store_row(G_* row, size_t first, unsigned G, size_t width,
+                                          const float (&v)[N]) {
+  // as many elements of G_ as fit 16 bytes at a time
+  constexpr int SW = VW * sizeof(G_) > 16 ? 16 / sizeof(G_) : VW;
+#pragma unroll
+  for (int k = 0; k < N / VW; k++) {
+    const size_t c = first + (size_t)k * G * VW;
+    if (c < width) {
+#pragma unroll
+      for (int h = 0; h < VW / SW; h++) {
+        Chunk<G_, SW> o;
+#pragma unroll
+        for (int e = 0; e < SW; e++) o.x[e] = from_f32<G_>(v[k * VW + h * SW + e]);
+        *reinterpret_cast<Chunk<G_, SW>*>(row + c + h * SW) = o;
       }
-      __syncthreads();
     }
-    if (col < width) {
-      G* o = gw + (size_t)v * width + col;
-      const float r = fmul(acc, scale);
-      if (!accumulate) *o = from_f32<G>(r);
-      else if (any) *o = from_f32<G>(fadd(to_f32(*o), r));
+  }
+}
+
+// v[e] = old + v[e].
+template <int VW, class G_, int N>
+__device__ __forceinline__ void add_row(const G_* row, size_t first, unsigned G, size_t width,
+                                        float (&v)[N]) {
+  constexpr int SW = VW * sizeof(G_) > 16 ? 16 / sizeof(G_) : VW;
+#pragma unroll
+  for (int k = 0; k < N / VW; k++) {
+    const size_t c = first + (size_t)k * G * VW;
+    if (c < width) {
+#pragma unroll
+      for (int h = 0; h < VW / SW; h++) {
+        const auto o = *reinterpret_cast<const Chunk<G_, SW>*>(row + c + h * SW);
+#pragma unroll
+        for (int e = 0; e < SW; e++) {
+          float& x = v[k * VW + h * SW + e];
+          x = fadd(to_f32(o.x[e]), x);
+        }
+      }
     }
+  }
+}
+
+// ---- forward -------------------------------------------------------------------
+
+// R rows to a group, one tile of G * 16 bytes of each.
+template <class T, int VW, int R>
+__global__ void __launch_bounds__(kThreads)
+embedding_kernel(const T* w, IndexArray ids, size_t n, long long vocab, size_t width, float scale,
+                 T* out, int* bad, unsigned G, unsigned tiles) {
+  constexpr int N = Row<T>::N;
+  const unsigned per_block = kThreads / G;
+  const size_t unit = (size_t)blockIdx.x * per_block + threadIdx.x / G;
+  const size_t i0 = unit / tiles * R;
+  const unsigned lane = threadIdx.x % G;
+  const size_t first = (size_t)(unit % tiles) * G * N + (size_t)lane * VW;
+  Row<T> x[R];
+  bool good[R];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    good[r] = false;
+    if (i0 + r < n) {
+      const long long id = ids[i0 + r];
+      good[r] = id >= 0 && id < vocab;
+      if (good[r]) load_row<VW, false>(w + (size_t)id * width, first, G, width, x[r]);
+      else if (first == 0) atomicExch(bad, 1);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    if (i0 + r < n) {
+      float v[N];
+#pragma unroll
+      for (int e = 0; e < N; e++)
+        v[e] = good[r] ? fmul(to_f32(x[r].x[e]), scale) : u2f(0x7fc00000u);
+      store_row<VW>(out + (i0 + r) * width, first, G, width, v);
+    }
+  }
+}
+
+// Threads that share a row: as many as it has 16-byte parts, at most a block.
+unsigned group_of(size_t width, int n_per_thread) {
+  unsigned g = 8;
+  while (g < (unsigned)kThreads && (size_t)g * n_per_thread < width) g *= 2;
+  return g;
+}
+
+// The widest chunk (in elements, at most 16 bytes) that every row start of
+// these tensors allows.
+template <class T>
+int chunk_of(size_t width, const void* a, size_t a_size, const void* b, size_t b_size) {
+  int vw = 16 / (int)sizeof(T);
+  while (vw > 1 && (width % vw ||
+                    reinterpret_cast<uintptr_t>(a) % std::min<size_t>(16, vw * a_size) ||
+                    reinterpret_cast<uintptr_t>(b) % std::min<size_t>(16, vw * b_size)))
+    vw /= 2;
+  return vw;
+}
+
+template <class T, int VW>
+cudaError_t embedding_of(const T* w, IndexArray ids, size_t n, size_t vocab, size_t width,
+                         float scale, T* out, int* bad, cudaStream_t s) {
+  constexpr int N = Row<T>::N;
+  const unsigned G = group_of(width, N);
+  const unsigned tiles = (unsigned)((width + (size_t)G * N - 1) / ((size_t)G * N));
+  const unsigned per_block = kThreads / G;
+  // Four rows a group keep 64 bytes a thread in flight; with few rows one each
+  // spreads them over more SMs.
+  int device = 0;
+  cudaGetDevice(&device);
+  const bool many = n * tiles >= (size_t)8 * sm_count(device) * per_block;
+  const size_t units = (many ? (n + 3) / 4 : n) * tiles;
+  const size_t blocks = (units + per_block - 1) / per_block;
+  if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
+  if (many)
+    embedding_kernel<T, VW, 4><<<(unsigned)blocks, kThreads, 0, s>>>(
+        w, ids, n, (long long)vocab, width, scale, out, bad, G, tiles);
+  else
+    embedding_kernel<T, VW, 1><<<(unsigned)blocks, kThreads, 0, s>>>(
+        w, ids, n, (long long)vocab, width, scale, out, bad, G, tiles);
+  return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t embedding_any(const void* weight, IndexArray ids, size_t n, size_t vocab, size_t width,
+                          float scale, void* out, int* bad, cudaStream_t s) {
+  const T* w = static_cast<const T*>(weight);
+  T* o = static_cast<T*>(out);
+  switch (chunk_of<T>(width, w, sizeof(T), o, sizeof(T))) {
+    case 8:
+      if constexpr (sizeof(T) == 2)
+        return embedding_of<T, 8>(w, ids, n, vocab, width, scale, o, bad, s);
+    case 4: return embedding_of<T, 4>(w, ids, n, vocab, width, scale, o, bad, s);
+    case 2: return embedding_of<T, 2>(w, ids, n, vocab, width, scale, o, bad, s);
+    default: return embedding_of<T, 1>(w, ids, n, vocab, width, scale, o, bad, s);
+  }
+}
+
+// ---- sorting ---------------------------------------------------------------------
+
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortMaxCluster = 8;
+constexpr int kSortMaxBits = 9;
+
+struct Sorted {
+  unsigned* key[2];     // [n] each: sorted keys end up in key[passes & 1]
+  unsigned* pos[2];     // [n] each: where in ids they were
+  unsigned* present;    // one bit per id
+  unsigned* crossing;   // [0]: how many pieces start a sum that crosses their end
+};
+
+__device__ __forceinline__ unsigned key_of(const IndexArray& ids, size_t i, long long vocab,
+                                           long long padding, int* bad) {
+  const long long id = ids[i];
+  if (id < 0 || id >= vocab) {
+    atomicExch(bad, 1);
+    return (unsigned)vocab;
+  }
+  return id == padding ? (unsigned)vocab : (unsigned)id;
+}
+
+// Stable least-significant-digit radix sort of n keys below 2^(bits * passes)
+// by one cluster.  Every warp owns a contiguous range of the list.  A pass
+// counts each warp's digits, turns the counts into where each warp's first key
+// of each digit goes (over warps, then the cluster's blocks through
+// distributed shared memory, then digits), and moves the keys, a warp's lanes
+// with the same digit in lane order.  Latency bounds it: n = 32768 is 4 keys a
+// thread, and the passes' barriers outweigh their loads.
+// Ids that have no row (outside the vocabulary, or padding) get key = vocab,
+// which sorts last.
+__global__ void __launch_bounds__(kSortThreads)
+sort_ids_kernel(IndexArray ids, unsigned n, long long vocab, long long padding, int bits,
+                int passes, Sorted out, int* bad) {
+  extern __shared__ unsigned hist[];                     // [kSortWarps][bins]
+  __shared__ unsigned block_total[1 << kSortMaxBits];    // read by the cluster
+  __shared__ unsigned warp_sum[kSortWarps];
+  cg::cluster_group cluster = cg::this_cluster();
+  const unsigned rank = cluster.block_rank(), blocks = cluster.num_blocks();
+  const unsigned bins = 1u << bits;
+  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned warps = blocks * kSortWarps;
+  const unsigned per_warp = ((n + warps - 1) / warps + 31) & ~31u;
+  const unsigned long long begin64 = (unsigned long long)(rank * kSortWarps + warp) * per_warp;
+  const unsigned begin = (unsigned)min(begin64, (unsigned long long)n);
+  const unsigned end = (unsigned)min(begin64 + per_warp, (unsigned long long)n);
+  unsigned* mine = hist + warp * bins;
+
+  const unsigned words = (unsigned)((vocab + 31) / 32);
+  for (unsigned i = rank * kSortThreads + threadIdx.x; i < words; i += blocks * kSortThreads)
+    out.present[i] = 0;
+  if (rank == 0 && threadIdx.x == 0) out.crossing[0] = 0;
+
+  for (int pass = 0; pass < passes; pass++) {
+    const int shift = pass * bits;
+    const unsigned* kin = out.key[pass & 1];
+    const unsigned* pin = out.pos[pass & 1];
+    unsigned* kout = out.key[(pass + 1) & 1];
+    unsigned* pout = out.pos[(pass + 1) & 1];
+    for (unsigned b = threadIdx.x; b < kSortWarps * bins; b += kSortThreads) hist[b] = 0;
+    __syncthreads();
+    for (unsigned i = begin + lane; i < end; i += 32) {
+      const unsigned k = pass ? __ldcg(kin + i) : key_of(ids, i, vocab, padding, bad);
+      atomicAdd(&mine[(k >> shift) & (bins - 1)], 1u);
+    }
+    __syncthreads();
+    // over the block's warps: exclusive prefix of each digit
+    const unsigned b = threadIdx.x;
+    if (b < bins) {
+      unsigned sum = 0;
+      for (int w = 0; w < kSortWarps; w++) {
+        const unsigned c = hist[w * bins + b];
+        hist[w * bins + b] = sum;
+        sum += c;
+      }
+      block_total[b] = sum;
+    }
+    cluster.sync();
+    // over the cluster's blocks, then over digits
+    unsigned before = 0, all = 0;
+    if (b < bins) {
+      for (unsigned r = 0; r < blocks; r++) {
+        const unsigned c = *cluster.map_shared_rank(&block_total[b], r);
+        if (r < rank) before += c;
+        all += c;
+      }
+    }
+    unsigned scan = all;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned o = __shfl_up_sync(0xffffffffu, scan, d);
+      if (lane >= (unsigned)d) scan += o;
+    }
+    if (lane == 31) warp_sum[warp] = scan;
+    __syncthreads();
+    unsigned lower = 0;
+    for (unsigned w = 0; w < warp; w++) lower += warp_sum[w];
+    const unsigned base = lower + scan - all + before;
+    if (b < bins)
+      for (int w = 0; w < kSortWarps; w++) hist[w * bins + b] += base;
+    __syncthreads();
+    for (unsigned i0 = begin; i0 < end; i0 += 32) {
+      const unsigned i = i0 + lane;
+      const bool live = i < end;
+      const unsigned k = !live ? 0 : pass ? __ldcg(kin + i) : key_of(ids, i, vocab, padding, bad);
+      const unsigned p = !live ? 0 : pass ? __ldcg(pin + i) : i;
+      const unsigned digit = live ? (k >> shift) & (bins - 1) : bins;
+      const unsigned same = __match_any_sync(0xffffffffu, digit);
+      const unsigned rank_in = __popc(same & ((1u << lane) - 1));
+      unsigned to = 0;
+      if (live) to = mine[digit] + rank_in;
+      __syncwarp();
+      if (live && rank_in == 0) mine[digit] += __popc(same);
+      __syncwarp();
+      if (live) {
+        kout[to] = k;
+        pout[to] = p;
+        if (pass == 0 && k < vocab) {
+          unsigned* word = out.present + (k >> 5);
+          const unsigned bit = 1u << (k & 31);
+          if (!(__ldcg(word) & bit)) atomicOr(word, bit);
+        }
+      }
+    }
+    __threadfence();
+    cluster.sync();   // the keys have arrived, and block_total may be overwritten
+  }
+}
+
+// ---- sums -------------------------------------------------------------------------
+
+constexpr int kSub = 32;             // sorted positions whose ids are staged at a time
+constexpr int kMinPiece = 32;
+constexpr size_t kMaxPieces = 2048;
+
+struct Plan {
+  unsigned n, piece, pieces;
+  const unsigned *key, *pos, *present;
+  unsigned* crossing;     // [0] count, [1 + e] the pieces
+  float* partial;         // [pieces][2][ld]: a sum that began before the piece; one that ends later
+  size_t ld;
+  long long vocab;
+  size_t width;
+  float scale;
+  bool accumulate;
+  unsigned G, tiles, per_block;
+  unsigned sum_blocks;    // then blocks that write zeros
+  unsigned zero_rows;     // rows of the table for each of those
+};
+
+template <int VW, class W, int N>
+__device__ __forceinline__ void write_sum(const Plan& a, W* gw, unsigned id, size_t first,
+                                          const float (&acc)[N]) {
+  float v[N];
+#pragma unroll
+  for (int e = 0; e < N; e++) v[e] = fmul(acc[e], a.scale);
+  W* row = gw + (size_t)id * a.width;
+  if (a.accumulate) add_row<VW>(row, first, a.G, a.width, v);
+  store_row<VW>(row, first, a.G, a.width, v);
+}
+
+template <class W>
+__device__ __forceinline__ void write_zeros(const Plan& a, W* gw) {
+  const long long v0 = (long long)(blockIdx.x - a.sum_blocks) * a.zero_rows;
+  const long long v1 = min(v0 + (long long)a.zero_rows, a.vocab);
+  for (long long v = v0; v < v1; v++) {
+    if ((a.present[v >> 5] >> (v & 31)) & 1u) continue;
+    W* row = gw + (size_t)v * a.width;
+    // 16-byte stores from the first 16-byte boundary on
+    const unsigned head = (unsigned)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(W));
+    const size_t lead = min((size_t)head, a.width);
+    const size_t vecs = (a.width - lead) * sizeof(W) / 16;
+    for (size_t c = threadIdx.x; c < lead; c += kThreads) row[c] = from_f32<W>(0.0f);
+    uint4* q = reinterpret_cast<uint4*>(row + lead);
+    for (size_t c = threadIdx.x; c < vecs; c += kThreads) __stcs(q + c, make_uint4(0, 0, 0, 0));
+    for (size_t c = lead + vecs * (16 / sizeof(W)) + threadIdx.x; c < a.width; c += kThreads)
+      row[c] = from_f32<W>(0.0f);
+  }
+}
+
+// U rows' loads in flight per thread.
+template <class T, class W, int VW>
+__global__ void __launch_bounds__(kThreads)
+segment_kernel(const T* g, W* gw, Plan a) {
+  constexpr int N = Row<T>::N;
+  constexpr int U = 8;
+  if (blockIdx.x >= a.sum_blocks) {
+    write_zeros(a, gw);
+    return;
+  }
+  extern __shared__ unsigned staged[];   // per group: kSub keys, then kSub positions
+  const unsigned group = threadIdx.x / a.G, lane = threadIdx.x % a.G;
+  unsigned* skey = staged + group * 2 * kSub;
+  unsigned* spos = skey + kSub;
+  const size_t unit = (size_t)blockIdx.x * a.per_block + group;
+  const unsigned piece = (unsigned)(unit / a.tiles);
+  const size_t first = (size_t)(unit % a.tiles) * a.G * N + (size_t)lane * VW;
+  const bool live = piece < a.pieces;
+  const unsigned p0 = live ? piece * a.piece : a.n;
+  const unsigned p1 = live ? min(p0 + a.piece, a.n) : a.n;
+  const unsigned none = (unsigned)a.vocab;
+
+  float acc[N];
+#pragma unroll
+  for (int e = 0; e < N; e++) acc[e] = 0.0f;
+  unsigned cur = live ? a.key[p0] : none;
+  bool head = live && p0 > 0 && a.key[p0 - 1] == cur;   // cur's sum began in an earlier piece
+  float* part = a.partial + (size_t)piece * 2 * a.ld + first;
+
+  auto put_partial = [&](int which) {
+    float* o = part + which * a.ld;
+#pragma unroll
+    for (int k = 0; k < N / VW; k++)
+#pragma unroll
+      for (int e = 0; e < VW; e++) {
+        const size_t c = (size_t)k * a.G * VW + e;
+        if (first + c < a.width) o[c] = acc[k * VW + e];
+      }
+  };
+
+  // every group of the block takes the same number of turns
+  for (unsigned s0 = 0; s0 < a.piece; s0 += kSub) {
+    __syncthreads();
+    for (unsigned i = lane; i < kSub; i += a.G) {
+      const unsigned p = p0 + s0 + i;
+      skey[i] = p < p1 ? a.key[p] : none;
+      spos[i] = p < p1 ? a.pos[p] : 0;
+    }
+    __syncthreads();
+    for (unsigned i = 0; i < kSub; i += U) {
+      Row<T> x[U];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (skey[i + u] != none)
+          load_row<VW, true>(g + (size_t)spos[i + u] * a.width, first, a.G, a.width, x[u]);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const unsigned k = skey[i + u];
+        if (k != cur) {
+          if (cur != none) {
+            if (head) put_partial(0);
+            else write_sum<VW>(a, gw, cur, first, acc);
+          }
+          head = false;
+          cur = k;
+#pragma unroll
+          for (int e = 0; e < N; e++) acc[e] = 0.0f;
+        }
+        if (k != none) {
+#pragma unroll
+          for (int e = 0; e < N; e++) acc[e] = fadd(acc[e], to_f32(x[u].x[e]));
+        }
+      }
+    }
+  }
+  // the last sum, unless padding or the end of the list closed it above
+  if (cur != none) {
+    const bool more = p1 < a.n && a.key[p1] == cur;
+    if (head) put_partial(0);
+    else if (more) put_partial(1);
+    else write_sum<VW>(a, gw, cur, first, acc);
+    if (!head && more && first == 0) a.crossing[1 + atomicAdd(a.crossing, 1u)] = piece;
+  }
+}
+
+// One sum that crosses pieces and 128 columns of it at a time: eight groups of
+// 32 threads add the partial sums of an eighth of the pieces each, in order,
+// then the eight are added in order.  The list's order does not matter.
+template <class W>
+__global__ void __launch_bounds__(kThreads) join_kernel(W* gw, Plan a) {
+  __shared__ float4 eighth[8][32];
+  const unsigned part = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned tiles = (unsigned)((a.width + 127) / 128);
+  const size_t items = (size_t)a.crossing[0] * tiles;
+  for (size_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const unsigned piece = a.crossing[1 + item / tiles];
+    const size_t c = (item % tiles) * 128 + lane * 4;
+    const unsigned id = a.key[piece * a.piece + a.piece - 1];
+    // how many pieces after this one hold the id: the last whose first key is
+    // still it (keys are sorted)
+    unsigned lo = piece + 1, hi = a.pieces - 1;
+    while (lo < hi) {
+      const unsigned mid = (lo + hi + 1) >> 1;
+      if (a.key[mid * a.piece] == id) lo = mid;
+      else hi = mid - 1;
+    }
+    const unsigned count = lo - piece + 1;   // partial sums: the first one's tail, then heads
+    const unsigned each = (count + 7) / 8;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const unsigned j1 = min((part + 1) * each, count);
+    if (c < a.width) {
+#pragma unroll 4
+      for (unsigned j = part * each; j < j1; j++) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(
+            a.partial + (size_t)(piece + j) * 2 * a.ld + (j == 0 ? a.ld : 0) + c));
+        acc.x = fadd(acc.x, x.x);
+        acc.y = fadd(acc.y, x.y);
+        acc.z = fadd(acc.z, x.z);
+        acc.w = fadd(acc.w, x.w);
+      }
+    }
+    eighth[part][lane] = acc;
+    __syncthreads();
+    if (part == 0 && c < a.width) {
+      for (int k = 1; k < 8; k++) {
+        const float4 x = eighth[k][lane];
+        acc.x = fadd(acc.x, x.x);
+        acc.y = fadd(acc.y, x.y);
+        acc.z = fadd(acc.z, x.z);
+        acc.w = fadd(acc.w, x.w);
+      }
+      const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+      W* row = gw + (size_t)id * a.width;
+      for (int e = 0; e < 4; e++)
+        if (c + e < a.width) {
+          const float r = fmul(v[e], a.scale);
+          row[c + e] = from_f32<W>(a.accumulate ? fadd(to_f32(row[c + e]), r) : r);
+        }
+    }
+    __syncthreads();
+  }
+}
+
+size_t up256(size_t b) { return (b + 255) & ~size_t(255); }
+
+struct Layout {
+  unsigned piece, pieces;
+  size_t ld, list, bitmap, crossing, partial, total;
+};
+Layout layout_of(size_t n, size_t vocab, size_t width) {
+  Layout l;
+  size_t piece = kMinPiece;
+  while ((n + piece - 1) / piece > kMaxPieces) piece *= 2;
+  l.piece = (unsigned)piece;
+  l.pieces = (unsigned)((n + piece - 1) / piece);
+  l.ld = (width + 3) & ~size_t(3);
+  l.list = up256(n * 4);
+  l.bitmap = up256((vocab + 31) / 32 * 4);
+  l.crossing = up256(((size_t)l.pieces + 1) * 4);
+  l.partial = (size_t)l.pieces * 2 * l.ld * 4;
+  l.total = 4 * l.list + l.bitmap + l.crossing + l.partial;
+  return l;
+}
+
+cudaError_t sort_ids(IndexArray ids, unsigned n, size_t vocab, long long padding,
+                     const Sorted& out, int* bad, int* passes_out, cudaStream_t s) {
+  int total_bits = 1;
+  while (total_bits < 32 && (vocab >> total_bits)) total_bits++;
+  const int passes = (total_bits + kSortMaxBits - 1) / kSortMaxBits;
+  const int bits = (total_bits + passes - 1) / passes;
+  // about 128 keys a warp before another block joins
+  unsigned blocks = 1;
+  while (blocks < kSortMaxCluster && (size_t)blocks * kSortWarps * 128 < n) blocks *= 2;
+  const size_t smem = (size_t)kSortWarps * (1u << bits) * 4;
+  cudaError_t e = cudaFuncSetAttribute(
+      sort_ids_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      kSortWarps * (1 << kSortMaxBits) * 4);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  *passes_out = passes;
+  return cudaLaunchKernelEx(&cfg, sort_ids_kernel, ids, n, (long long)vocab, padding, bits, passes,
+                            out, bad);
+}
+
+template <class T, class W, int VW>
+cudaError_t sums_of(const void* g, void* gw, Plan a, cudaStream_t s) {
+  constexpr int N = Row<T>::N;
+  a.G = group_of(a.width, N);
+  a.tiles = (unsigned)((a.width + (size_t)a.G * N - 1) / ((size_t)a.G * N));
+  a.per_block = kThreads / a.G;
+  const size_t units = (size_t)a.pieces * a.tiles;
+  const size_t sum_blocks = (units + a.per_block - 1) / a.per_block;
+  size_t zero_blocks = 0;
+  if (!a.accumulate) {
+    // 128 KB of the table to a block that writes zeros
+    const size_t row = a.width * sizeof(W);
+    a.zero_rows = (unsigned)std::max<size_t>(1, std::min<size_t>((size_t)131072 / row, 1u << 20));
+    zero_blocks = ((size_t)a.vocab + a.zero_rows - 1) / a.zero_rows;
+  }
+  if (sum_blocks + zero_blocks > 0x7fffffffull) return cudaErrorInvalidValue;
+  a.sum_blocks = (unsigned)sum_blocks;
+  const size_t smem = (size_t)a.per_block * 2 * kSub * 4;
+  segment_kernel<T, W, VW><<<(unsigned)(sum_blocks + zero_blocks), kThreads, smem, s>>>(
+      static_cast<const T*>(g), static_cast<W*>(gw), a);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || a.pieces < 2) return e;
+  join_kernel<W><<<(unsigned)std::min<size_t>((size_t)a.pieces * ((a.width + 127) / 128), 592),
+                   kThreads, 0, s>>>(static_cast<W*>(gw), a);
+  return cudaGetLastError();
+}
+
+template <class T, class W>
+cudaError_t sums_any(const void* g, void* gw, const Plan& a, cudaStream_t s) {
+  switch (chunk_of<T>(a.width, g, sizeof(T), gw, sizeof(W))) {
+    case 8:
+      if constexpr (sizeof(T) == 2) return sums_of<T, W, 8>(g, gw, a, s);
+    case 4: return sums_of<T, W, 4>(g, gw, a, s);
+    case 2: return sums_of<T, W, 2>(g, gw, a, s);
+    default: return sums_of<T, W, 1>(g, gw, a, s);
   }
 }
 
@@ -71,59 +626,67 @@ cudaError_t launch_embedding(StoreType t, const void* weight, const void* ids, b
                              size_t n, size_t vocab, size_t width, float scale, void* out,
                              int* bad, cudaStream_t s) {
   if (n == 0 || width == 0) return cudaSuccess;
-  const unsigned grid = (unsigned)std::min<size_t>(n, 1u << 20);
   const IndexArray ia{ids, wide};
   switch (t) {
-    case kF32:
-      embedding_kernel<float><<<grid, kThreads, 0, s>>>((const float*)weight, ia, n, vocab, width,
-                                                        scale, (float*)out, bad);
-      break;
-    case kBF16:
-      embedding_kernel<bf16><<<grid, kThreads, 0, s>>>((const bf16*)weight, ia, n, vocab, width,
-                                                       scale, (bf16*)out, bad);
-      break;
-    case kF16:
-      embedding_kernel<f16><<<grid, kThreads, 0, s>>>((const f16*)weight, ia, n, vocab, width,
-                                                      scale, (f16*)out, bad);
-      break;
+    case kF32: return embedding_any<float>(weight, ia, n, vocab, width, scale, out, bad, s);
+    case kBF16: return embedding_any<bf16>(weight, ia, n, vocab, width, scale, out, bad, s);
+    case kF16: return embedding_any<f16>(weight, ia, n, vocab, width, scale, out, bad, s);
   }
-  return cudaGetLastError();
+  return cudaErrorInvalidValue;
 }
 
-size_t embedding_backward_scratch(size_t, size_t, size_t) { return 256; }
-
-namespace {
-template <class T, class G>
-cudaError_t backward_of(const void* g, IndexArray ids, size_t n, size_t vocab, size_t width,
-                        float scale, long long padding, bool accumulate, void* gw, int* bad,
-                        cudaStream_t s) {
-  const dim3 grid((unsigned)std::min<size_t>(vocab, 1u << 20),
-                  (unsigned)((width + kThreads - 1) / kThreads));
-  embedding_backward_kernel<T, G><<<grid, kThreads, 0, s>>>(
-      (const T*)g, ids, n, vocab, width, scale, padding, accumulate, (G*)gw, bad);
-  return cudaGetLastError();
+size_t embedding_backward_scratch(size_t n, size_t vocab, size_t width) {
+  return layout_of(n, vocab, width).total;
 }
-}  // namespace
 
 cudaError_t launch_embedding_backward(StoreType t, const void* grad_output, const void* ids,
                                       bool wide, size_t n, size_t vocab, size_t width,
                                       float scale, long long padding, bool accumulate,
-                                      void* grad_weight, bool narrow, void*, int* bad,
+                                      void* grad_weight, bool narrow, void* scratch, int* bad,
                                       cudaStream_t s) {
   if (vocab == 0 || width == 0) return cudaSuccess;
-  const IndexArray ia{ids, wide};
-  if (t == kF32)
-    return backward_of<float, float>(grad_output, ia, n, vocab, width, scale, padding, accumulate,
-                                     grad_weight, bad, s);
-  if (t == kBF16)
-    return narrow ? backward_of<bf16, bf16>(grad_output, ia, n, vocab, width, scale, padding,
-                                            accumulate, grad_weight, bad, s)
-                  : backward_of<bf16, float>(grad_output, ia, n, vocab, width, scale, padding,
-                                             accumulate, grad_weight, bad, s);
-  return narrow ? backward_of<f16, f16>(grad_output, ia, n, vocab, width, scale, padding,
-                                        accumulate, grad_weight, bad, s)
-                : backward_of<f16, float>(grad_output, ia, n, vocab, width, scale, padding,
-                                          accumulate, grad_weight, bad, s);
+  if (n == 0)
+    return accumulate ? cudaSuccess
+                      : cudaMemsetAsync(grad_weight, 0,
+                                        vocab * width * (narrow ? store_bytes(t) : 4), s);
+  const Layout l = layout_of(n, vocab, width);
+  char* p = static_cast<char*>(scratch);
+  Sorted sorted;
+  sorted.key[0] = reinterpret_cast<unsigned*>(p);
+  sorted.key[1] = reinterpret_cast<unsigned*>(p + l.list);
+  sorted.pos[0] = reinterpret_cast<unsigned*>(p + 2 * l.list);
+  sorted.pos[1] = reinterpret_cast<unsigned*>(p + 3 * l.list);
+  p += 4 * l.list;
+  sorted.present = reinterpret_cast<unsigned*>(p);
+  sorted.crossing = reinterpret_cast<unsigned*>(p + l.bitmap);
+  int passes = 0;
+  const cudaError_t e = sort_ids(IndexArray{ids, wide}, (unsigned)n, vocab, padding, sorted, bad,
+                                 &passes, s);
+  if (e != cudaSuccess) return e;
+  Plan a = {};
+  a.n = (unsigned)n;
+  a.piece = l.piece;
+  a.pieces = l.pieces;
+  a.key = sorted.key[passes & 1];
+  a.pos = sorted.pos[passes & 1];
+  a.present = sorted.present;
+  a.crossing = sorted.crossing;
+  a.partial = reinterpret_cast<float*>(p + l.bitmap + l.crossing);
+  a.ld = l.ld;
+  a.vocab = (long long)vocab;
+  a.width = width;
+  a.scale = scale;
+  a.accumulate = accumulate;
+  switch (t) {
+    case kF32: return sums_any<float, float>(grad_output, grad_weight, a, s);
+    case kBF16:
+      return narrow ? sums_any<bf16, bf16>(grad_output, grad_weight, a, s)
+                    : sums_any<bf16, float>(grad_output, grad_weight, a, s);
+    case kF16:
+      return narrow ? sums_any<f16, f16>(grad_output, grad_weight, a, s)
+                    : sums_any<f16, float>(grad_output, grad_weight, a, s);
+  }
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace rt
