@@ -145,7 +145,7 @@ extern "C" rtc_result rtc_embedding_backward(const rtc_tensor* grad_output, cons
   TRY(apart(grad_weight, grad_output, "grad_weight"));
   TRY(apart(grad_weight, ids, "grad_weight"));
   if (grad_weight->numel == 0) return ok();
-  return on_device(grad_output->device, embedding_backward_scratch(ids->numel, vocab, width), ctx,
+  return on_device(grad_output->device, embedding_backward_scratch(ids->numel, width), ctx,
                    [&](void* scratch, int* bad) {
                      return launch_embedding_backward(
                          type, grad_output->data, ids->data, ids->dtype == RTC_I64, ids->numel,

@@ -6,7 +6,7 @@
 // Gradient: grad_weight[v, :] (+)= scale * sum over {i : ids[i] = v} of
 // grad_output[i, :].  The sums of a row are wherever its tokens are, so:
 //  1. sort_ids_kernel sorts the positions by id (stable radix sort) in one
-//     cluster of thread blocks, and marks which ids occur;
+//     cluster of thread blocks;
 //  2. segment_kernel cuts the sorted list into pieces of equal length, so
 //     that a frequent id costs no block more than a rare one; a group sums its
 //     piece's rows in order, writes each id's sum that begins and ends in the
@@ -16,6 +16,7 @@
 // No floating-point atomics: the order of every sum follows from ids alone.
 #include "rt_internal.h"
 #include "rt_libm.cuh"
+#include "rt_tma.cuh"
 #include "rt_types.cuh"
 
 #include <cooperative_groups.h>
@@ -213,10 +214,8 @@ constexpr int kSortMaxCluster = 8;
 constexpr int kSortMaxBits = 9;
 
 struct Sorted {
-  unsigned* key[2];     // [n] each: sorted keys end up in key[passes & 1]
-  unsigned* pos[2];     // [n] each: where in ids they were
-  unsigned* present;    // one bit per id
-  unsigned* crossing;   // [0]: how many pieces start a sum that crosses their end
+  uint2* pair[2];       // [n] each: key, and where in ids it was; sorted in pair[passes & 1]
+  unsigned* count;      // [2]: of the sums that cross pieces, zeroed here
 };
 
 __device__ __forceinline__ unsigned key_of(const IndexArray& ids, size_t i, long long vocab,
@@ -231,18 +230,23 @@ __device__ __forceinline__ unsigned key_of(const IndexArray& ids, size_t i, long
 
 // Stable least-significant-digit radix sort of n keys below 2^(bits * passes)
 // by one cluster.  Every warp owns a contiguous range of the list.  A pass
-// counts each warp's digits, turns the counts into where each warp's first key
-// of each digit goes (over warps, then the cluster's blocks through
-// distributed shared memory, then digits), and moves the keys, a warp's lanes
-// with the same digit in lane order.  Latency bounds it: n = 32768 is 4 keys a
-// thread, and the passes' barriers outweigh their loads.
+// ranks each key among its warp's keys of the same digit (ballots over the
+// digit's bits give a lane its equals), turns the warps' counts into where
+// each warp's first key of each digit goes (over warps, then the cluster's
+// blocks through distributed shared memory, then digits), and moves the keys.
+// Latency bounds it, not bytes: with HELD a warp's 32 * K keys at most stay in
+// registers between ranking and moving, all of them loaded at once; longer
+// ranges are read twice.  A scattered store takes the SM a cycle for each
+// lane, so key and position travel as one, over all the blocks of a cluster.
 // Ids that have no row (outside the vocabulary, or padding) get key = vocab,
 // which sorts last.
+template <int K, bool HELD>
 __global__ void __launch_bounds__(kSortThreads)
 sort_ids_kernel(IndexArray ids, unsigned n, long long vocab, long long padding, int bits,
                 int passes, Sorted out, int* bad) {
   extern __shared__ unsigned hist[];                     // [kSortWarps][bins]
   __shared__ unsigned block_total[1 << kSortMaxBits];    // read by the cluster
+  __shared__ unsigned base[1 << kSortMaxBits];           // where the block's digits go
   __shared__ unsigned warp_sum[kSortWarps];
   cg::cluster_group cluster = cg::this_cluster();
   const unsigned rank = cluster.block_rank(), blocks = cluster.num_blocks();
@@ -254,29 +258,63 @@ sort_ids_kernel(IndexArray ids, unsigned n, long long vocab, long long padding, 
   const unsigned begin = (unsigned)min(begin64, (unsigned long long)n);
   const unsigned end = (unsigned)min(begin64 + per_warp, (unsigned long long)n);
   unsigned* mine = hist + warp * bins;
+  if (rank == 0 && threadIdx.x < 2) out.count[threadIdx.x] = 0;
 
-  const unsigned words = (unsigned)((vocab + 31) / 32);
-  for (unsigned i = rank * kSortThreads + threadIdx.x; i < words; i += blocks * kSortThreads)
-    out.present[i] = 0;
-  if (rank == 0 && threadIdx.x == 0) out.crossing[0] = 0;
-
+  auto clear_mine = [&] {
+    __syncwarp();
+    for (unsigned b = lane; b < bins; b += 32) mine[b] = 0;
+    __syncwarp();
+  };
+  clear_mine();
+  unsigned key[K], pos[K], to[K];
   for (int pass = 0; pass < passes; pass++) {
     const int shift = pass * bits;
-    const unsigned* kin = out.key[pass & 1];
-    const unsigned* pin = out.pos[pass & 1];
-    unsigned* kout = out.key[(pass + 1) & 1];
-    unsigned* pout = out.pos[(pass + 1) & 1];
-    for (unsigned b = threadIdx.x; b < kSortWarps * bins; b += kSortThreads) hist[b] = 0;
-    __syncthreads();
-    for (unsigned i = begin + lane; i < end; i += 32) {
-      const unsigned k = pass ? __ldcg(kin + i) : key_of(ids, i, vocab, padding, bad);
-      atomicAdd(&mine[(k >> shift) & (bins - 1)], 1u);
+    const uint2* in = out.pair[pass & 1];
+    uint2* moved = out.pair[(pass + 1) & 1];
+    auto load = [&](unsigned from) {
+#pragma unroll
+      for (int j = 0; j < K; j++) {
+        const unsigned i = from + j * 32 + lane;
+        key[j] = 0;
+        if (i < end) {
+          const uint2 x =
+              pass ? __ldcg(in + i) : make_uint2(key_of(ids, i, vocab, padding, bad), i);
+          key[j] = x.x;
+          pos[j] = x.y;
+        }
+      }
+    };
+    // to[j]: how many of the warp's keys before this one have its digit, on
+    // top of what `mine` starts with
+    auto rank_keys = [&](unsigned from) {
+#pragma unroll
+      for (int j = 0; j < K; j++) {
+        if (from + j * 32 >= end) break;        // the warp's lanes agree
+        const bool live = from + j * 32 + lane < end;
+        const unsigned digit = (key[j] >> shift) & (bins - 1);
+        unsigned same = __ballot_sync(0xffffffffu, live);
+#pragma unroll
+        for (int d = 0; d < kSortMaxBits; d++) {   // bits above `bits` are 0 in every lane
+          const unsigned m = __ballot_sync(0xffffffffu, (digit >> d) & 1u);
+          same &= (digit >> d) & 1u ? m : ~m;
+        }
+        const unsigned before = __popc(same & ((1u << lane) - 1));
+        if (live) to[j] = mine[digit] + before;
+        __syncwarp();
+        if (live && before == 0) mine[digit] += __popc(same);
+        __syncwarp();
+      }
+    };
+    for (unsigned i0 = begin; i0 < end; i0 += 32 * K) {
+      load(i0);
+      rank_keys(i0);
     }
     __syncthreads();
     // over the block's warps: exclusive prefix of each digit
     const unsigned b = threadIdx.x;
     if (b < bins) {
       unsigned sum = 0;
+#pragma unroll
       for (int w = 0; w < kSortWarps; w++) {
         const unsigned c = hist[w * bins + b];
         hist[w * bins + b] = sum;
@@ -288,10 +326,13 @@ sort_ids_kernel(IndexArray ids, unsigned n, long long vocab, long long padding, 
     // over the cluster's blocks, then over digits
     unsigned before = 0, all = 0;
     if (b < bins) {
-      for (unsigned r = 0; r < blocks; r++) {
-        const unsigned c = *cluster.map_shared_rank(&block_total[b], r);
-        if (r < rank) before += c;
-        all += c;
+#pragma unroll
+      for (unsigned r = 0; r < kSortMaxCluster; r++) {
+        if (r < blocks) {
+          const unsigned c = *cluster.map_shared_rank(&block_total[b], r);
+          if (r < rank) before += c;
+          all += c;
+        }
       }
     }
     unsigned scan = all;
@@ -302,50 +343,52 @@ sort_ids_kernel(IndexArray ids, unsigned n, long long vocab, long long padding, 
     }
     if (lane == 31) warp_sum[warp] = scan;
     __syncthreads();
-    unsigned lower = 0;
-    for (unsigned w = 0; w < warp; w++) lower += warp_sum[w];
-    const unsigned base = lower + scan - all + before;
-    if (b < bins)
-      for (int w = 0; w < kSortWarps; w++) hist[w * bins + b] += base;
+    if (b < bins) {
+      unsigned at = scan - all + before;
+#pragma unroll
+      for (unsigned w = 0; w < (1u << kSortMaxBits) / 32; w++)
+        if (w < warp) at += warp_sum[w];
+      base[b] = at;
+    }
     __syncthreads();
-    for (unsigned i0 = begin; i0 < end; i0 += 32) {
-      const unsigned i = i0 + lane;
-      const bool live = i < end;
-      const unsigned k = !live ? 0 : pass ? __ldcg(kin + i) : key_of(ids, i, vocab, padding, bad);
-      const unsigned p = !live ? 0 : pass ? __ldcg(pin + i) : i;
-      const unsigned digit = live ? (k >> shift) & (bins - 1) : bins;
-      const unsigned same = __match_any_sync(0xffffffffu, digit);
-      const unsigned rank_in = __popc(same & ((1u << lane) - 1));
-      unsigned to = 0;
-      if (live) to = mine[digit] + rank_in;
-      __syncwarp();
-      if (live && rank_in == 0) mine[digit] += __popc(same);
-      __syncwarp();
-      if (live) {
-        kout[to] = k;
-        pout[to] = p;
-        if (pass == 0 && k < vocab) {
-          unsigned* word = out.present + (k >> 5);
-          const unsigned bit = 1u << (k & 31);
-          if (!(__ldcg(word) & bit)) atomicOr(word, bit);
+    for (unsigned i0 = begin; i0 < end; i0 += 32 * K) {
+      if (!HELD) {
+        load(i0);
+        rank_keys(i0);
+      }
+#pragma unroll
+      for (int j = 0; j < K; j++) {
+        if (i0 + j * 32 + lane < end) {
+          const unsigned digit = (key[j] >> shift) & (bins - 1);
+          // HELD: to[] counts from 0, the prefix over warps is in mine[]
+          const unsigned at = base[digit] + to[j] + (HELD ? mine[digit] : 0);
+          moved[at] = make_uint2(key[j], pos[j]);
         }
       }
     }
-    __threadfence();
-    cluster.sync();   // the keys have arrived, and block_total may be overwritten
+    // the keys have arrived, and block_total may be overwritten; a warp's
+    // counts are its own by now
+    cluster.barrier_arrive();
+    clear_mine();
+    cluster.barrier_wait();
   }
 }
 
 // ---- sums -------------------------------------------------------------------------
 
-constexpr int kSub = 32;             // sorted positions whose ids are staged at a time
+constexpr int kSub = 16;             // sorted positions whose ids are staged at a time
 constexpr int kMinPiece = 32;
 constexpr size_t kMaxPieces = 2048;
+constexpr unsigned kLong = 16;       // a sum over more pieces than this is a long one
+constexpr int kZeroRows = 64;        // at most, to a block that writes zeros
+constexpr int kZeroBytes = 4096;     // zeros that it copies at a time
 
 struct Plan {
   unsigned n, piece, pieces;
-  const unsigned *key, *pos, *present;
-  unsigned* crossing;     // [0] count, [1 + e] the pieces
+  const uint2* pair;      // sorted keys (.x) and positions
+  unsigned* count;        // [2]: sums that cross pieces, and of those the long ones apart
+  uint2* crossing;        // [pieces]: the piece where one begins, and its id
+  uint2* crossing_long;   // [pieces / kLong + 1]
   float* partial;         // [pieces][2][ld]: a sum that began before the piece; one that ends later
   size_t ld;
   long long vocab;
@@ -356,6 +399,10 @@ struct Plan {
   unsigned sum_blocks;    // then blocks that write zeros
   unsigned zero_rows;     // rows of the table for each of those
 };
+
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
 
 template <int VW, class W, int N>
 __device__ __forceinline__ void write_sum(const Plan& a, W* gw, unsigned id, size_t first,
@@ -368,31 +415,82 @@ __device__ __forceinline__ void write_sum(const Plan& a, W* gw, unsigned id, siz
   store_row<VW>(row, first, a.G, a.width, v);
 }
 
-template <class W>
-__device__ __forceinline__ void write_zeros(const Plan& a, W* gw) {
-  const long long v0 = (long long)(blockIdx.x - a.sum_blocks) * a.zero_rows;
-  const long long v1 = min(v0 + (long long)a.zero_rows, a.vocab);
-  for (long long v = v0; v < v1; v++) {
-    if ((a.present[v >> 5] >> (v & 31)) & 1u) continue;
-    W* row = gw + (size_t)v * a.width;
-    // 16-byte stores from the first 16-byte boundary on
-    const unsigned head = (unsigned)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(W));
-    const size_t lead = min((size_t)head, a.width);
-    const size_t vecs = (a.width - lead) * sizeof(W) / 16;
-    for (size_t c = threadIdx.x; c < lead; c += kThreads) row[c] = from_f32<W>(0.0f);
-    uint4* q = reinterpret_cast<uint4*>(row + lead);
-    for (size_t c = threadIdx.x; c < vecs; c += kThreads) __stcs(q + c, make_uint4(0, 0, 0, 0));
-    for (size_t c = lead + vecs * (16 / sizeof(W)) + threadIdx.x; c < a.width; c += kThreads)
-      row[c] = from_f32<W>(0.0f);
+// How many of the n sorted keys are below v: a warp looks at 32 places at a
+// time.
+__device__ __forceinline__ unsigned lower_bound(const uint2* key, unsigned n, unsigned v) {
+  const unsigned lane = threadIdx.x & 31;
+  unsigned lo = 0, hi = n;             // the answer is in [lo, hi]
+  while (lo < hi) {
+    const unsigned step = (hi - lo + 31) / 32;
+    const unsigned at = lo + lane * step;      // below 2^31 + 2^31
+    const unsigned below =
+        __popc(__ballot_sync(0xffffffffu, at < hi && key[at].x < v));   // a prefix of the lanes
+    if (below == 0) return lo;
+    const unsigned last = lo + (below - 1) * step;
+    hi = min(hi, last + step);
+    lo = last + 1;
   }
+  return lo;
 }
 
-// U rows' loads in flight per thread.
+template <class W>
+__device__ __forceinline__ void write_zeros(const Plan& a, W* gw) {
+  __shared__ unsigned here[kZeroRows / 32];      // the block's rows that have tokens
+  __shared__ unsigned range[2];
+  __shared__ uint4 zeros[kZeroBytes / 16];
+  for (int i = threadIdx.x; i < kZeroBytes / 16; i += kThreads) zeros[i] = make_uint4(0, 0, 0, 0);
+  const long long v0 = (long long)(blockIdx.x - a.sum_blocks) * a.zero_rows;
+  const int rows = (int)min((long long)a.zero_rows, a.vocab - v0);
+  if (threadIdx.x < kZeroRows / 32) here[threadIdx.x] = 0;
+  if (threadIdx.x < 64) {
+    const unsigned w = threadIdx.x >> 5;
+    const unsigned p = lower_bound(a.pair, a.n, (unsigned)v0 + (w ? rows : 0));
+    if ((threadIdx.x & 31) == 0) range[w] = p;
+  }
+  __syncthreads();
+  for (unsigned p = range[0] + threadIdx.x; p < range[1]; p += kThreads) {
+    const unsigned r = a.pair[p].x - (unsigned)v0;
+    atomicOr(&here[r >> 5], 1u << (r & 31));
+  }
+  fence_proxy_async_smem();
+  __syncthreads();
+  // Runs of rows without tokens, an eighth of the block's rows to a warp: the
+  // 16-byte-aligned inside of a run as bulk copies of a block of zeros (one
+  // instruction where stores would take one for each 512 bytes of a warp), the
+  // ends element by element.
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int each = (rows + kThreads / 32 - 1) / (kThreads / 32);
+  const int last = min((warp + 1) * each, rows);
+  auto taken = [&](int r) { return (here[r >> 5] >> (r & 31)) & 1u; };
+  for (int r = warp * each; r < last;) {
+    if (taken(r)) {
+      r++;
+      continue;
+    }
+    int e = r + 1;
+    while (e < last && !taken(e)) e++;
+    char* b0 = reinterpret_cast<char*>(gw + (size_t)(v0 + r) * a.width);
+    char* b1 = reinterpret_cast<char*>(gw + (size_t)(v0 + e) * a.width);
+    char* a0 = b0 + (-reinterpret_cast<intptr_t>(b0) & 15);
+    char* a1 = b1 - (reinterpret_cast<intptr_t>(b1) & 15);
+    if (a0 >= a1) a0 = a1 = b1;
+    for (W* q = reinterpret_cast<W*>(b0) + lane; reinterpret_cast<char*>(q) < a0; q += 32)
+      *q = from_f32<W>(0.0f);
+    for (W* q = reinterpret_cast<W*>(a1) + lane; reinterpret_cast<char*>(q) < b1; q += 32)
+      *q = from_f32<W>(0.0f);
+    for (char* q = a0 + (size_t)lane * sizeof zeros; q < a1; q += 32 * sizeof zeros)
+      bulk_store(q, zeros, (unsigned)min((ptrdiff_t)sizeof zeros, (ptrdiff_t)(a1 - q)));
+    r = e;
+  }
+  bulk_store_wait();   // `zeros` has been read
+}
+
+// U rows' loads in flight per thread (fewer where a row takes many narrow ones).
 template <class T, class W, int VW>
 __global__ void __launch_bounds__(kThreads)
 segment_kernel(const T* g, W* gw, Plan a) {
   constexpr int N = Row<T>::N;
-  constexpr int U = 8;
+  constexpr int U = VW * sizeof(T) >= 8 ? 8 : 4;
   if (blockIdx.x >= a.sum_blocks) {
     write_zeros(a, gw);
     return;
@@ -412,8 +510,8 @@ segment_kernel(const T* g, W* gw, Plan a) {
   float acc[N];
 #pragma unroll
   for (int e = 0; e < N; e++) acc[e] = 0.0f;
-  unsigned cur = live ? a.key[p0] : none;
-  bool head = live && p0 > 0 && a.key[p0 - 1] == cur;   // cur's sum began in an earlier piece
+  unsigned cur = live ? a.pair[p0].x : none;
+  bool head = live && p0 > 0 && a.pair[p0 - 1].x == cur;   // cur's sum began in an earlier piece
   float* part = a.partial + (size_t)piece * 2 * a.ld + first;
 
   auto put_partial = [&](int which) {
@@ -432,10 +530,17 @@ segment_kernel(const T* g, W* gw, Plan a) {
     __syncthreads();
     for (unsigned i = lane; i < kSub; i += a.G) {
       const unsigned p = p0 + s0 + i;
-      skey[i] = p < p1 ? a.key[p] : none;
-      spos[i] = p < p1 ? a.pos[p] : 0;
+      const uint2 x = p < p1 ? a.pair[p] : make_uint2(none, 0);
+      skey[i] = x.x;
+      spos[i] = x.y;
     }
     __syncthreads();
+    if (a.accumulate)
+      for (unsigned i = 0; i < kSub; i++) {
+        const unsigned k = skey[i];
+        if (k != none && (i == 0 || skey[i - 1] != k) && first < a.width)
+          prefetch_l2(gw + (size_t)k * a.width + first);
+      }
     for (unsigned i = 0; i < kSub; i += U) {
       Row<T> x[U];
 #pragma unroll
@@ -464,90 +569,102 @@ segment_kernel(const T* g, W* gw, Plan a) {
   }
   // the last sum, unless padding or the end of the list closed it above
   if (cur != none) {
-    const bool more = p1 < a.n && a.key[p1] == cur;
+    const bool more = p1 < a.n && a.pair[p1].x == cur;
     if (head) put_partial(0);
     else if (more) put_partial(1);
     else write_sum<VW>(a, gw, cur, first, acc);
-    if (!head && more && first == 0) a.crossing[1 + atomicAdd(a.crossing, 1u)] = piece;
+    if (!head && more && first == 0) {
+      const size_t far = (size_t)(piece + kLong) * a.piece;
+      const bool is_long = far < a.n && a.pair[far].x == cur;
+      const unsigned e = atomicAdd(a.count + is_long, 1u);
+      (is_long ? a.crossing_long : a.crossing)[e] = make_uint2(piece, cur);
+    }
   }
 }
 
-// One sum that crosses pieces and 128 columns of it at a time: eight groups of
-// 32 threads add the partial sums of an eighth of the pieces each, in order,
-// then the eight are added in order.  The list's order does not matter.
+// Joins the sums that cross pieces.  Most take a few pieces: a thread adds four
+// columns' partial sums in order, 1024 columns to a block.  The long ones (at
+// most pieces / kLong) get a block for each 128 columns: eight groups of 32
+// threads add an eighth of the pieces each, in order, then the eight are added
+// in order.  Which block takes which sum does not matter.
 template <class W>
-__global__ void __launch_bounds__(kThreads) join_kernel(W* gw, Plan a) {
+__global__ void __launch_bounds__(kThreads)
+join_kernel(W* gw, Plan a, unsigned short_tiles, unsigned long_tiles) {
   __shared__ float4 eighth[8][32];
   const unsigned part = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const unsigned tiles = (unsigned)((a.width + 127) / 128);
-  const size_t items = (size_t)a.crossing[0] * tiles;
-  for (size_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const unsigned piece = a.crossing[1 + item / tiles];
-    const size_t c = (item % tiles) * 128 + lane * 4;
-    const unsigned id = a.key[piece * a.piece + a.piece - 1];
-    // how many pieces after this one hold the id: the last whose first key is
-    // still it (keys are sorted)
-    unsigned lo = piece + 1, hi = a.pieces - 1;
-    while (lo < hi) {
-      const unsigned mid = (lo + hi + 1) >> 1;
-      if (a.key[mid * a.piece] == id) lo = mid;
-      else hi = mid - 1;
+  const unsigned longs = (a.pieces / kLong + 1) * long_tiles;
+  const bool is_long = blockIdx.x < longs;
+  const unsigned b = is_long ? blockIdx.x : blockIdx.x - longs;
+  const unsigned tiles = is_long ? long_tiles : short_tiles;
+  const unsigned e = b / tiles;
+  if (e >= a.count[is_long]) return;
+  const uint2 which = (is_long ? a.crossing_long : a.crossing)[e];
+  const unsigned piece = which.x;
+  // the pieces after this one whose first key is still the id (keys are
+  // sorted), 32 looked at together
+  unsigned count = 1;   // partial sums: the first one's tail, then heads
+  for (unsigned q = piece + 1; q < a.pieces; q += 32) {
+    const bool more = q + lane < a.pieces && a.pair[(size_t)(q + lane) * a.piece].x == which.y;
+    const unsigned m = __ballot_sync(0xffffffffu, more);
+    count += __popc(m);
+    if (m != 0xffffffffu) break;
+  }
+  const unsigned each = is_long ? (count + 7) / 8 : count;
+  const unsigned j0 = is_long ? part * each : 0, j1 = min(j0 + each, count);
+  const size_t c = is_long ? (size_t)(b % tiles) * 128 + lane * 4
+                           : (size_t)(b % tiles) * (kThreads * 4) + threadIdx.x * 4;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (c < a.width) {
+#pragma unroll 8
+    for (unsigned j = j0; j < j1; j++) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(
+          a.partial + (size_t)(piece + j) * 2 * a.ld + (j == 0 ? a.ld : 0) + c));
+      acc.x = fadd(acc.x, x.x);
+      acc.y = fadd(acc.y, x.y);
+      acc.z = fadd(acc.z, x.z);
+      acc.w = fadd(acc.w, x.w);
     }
-    const unsigned count = lo - piece + 1;   // partial sums: the first one's tail, then heads
-    const unsigned each = (count + 7) / 8;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    const unsigned j1 = min((part + 1) * each, count);
-    if (c < a.width) {
-#pragma unroll 4
-      for (unsigned j = part * each; j < j1; j++) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(
-            a.partial + (size_t)(piece + j) * 2 * a.ld + (j == 0 ? a.ld : 0) + c));
-        acc.x = fadd(acc.x, x.x);
-        acc.y = fadd(acc.y, x.y);
-        acc.z = fadd(acc.z, x.z);
-        acc.w = fadd(acc.w, x.w);
-      }
-    }
+  }
+  if (is_long) {
     eighth[part][lane] = acc;
     __syncthreads();
-    if (part == 0 && c < a.width) {
-      for (int k = 1; k < 8; k++) {
-        const float4 x = eighth[k][lane];
-        acc.x = fadd(acc.x, x.x);
-        acc.y = fadd(acc.y, x.y);
-        acc.z = fadd(acc.z, x.z);
-        acc.w = fadd(acc.w, x.w);
-      }
-      const float v[4] = {acc.x, acc.y, acc.z, acc.w};
-      W* row = gw + (size_t)id * a.width;
-      for (int e = 0; e < 4; e++)
-        if (c + e < a.width) {
-          const float r = fmul(v[e], a.scale);
-          row[c + e] = from_f32<W>(a.accumulate ? fadd(to_f32(row[c + e]), r) : r);
-        }
+    if (part != 0) return;
+#pragma unroll
+    for (int k = 1; k < 8; k++) {
+      const float4 x = eighth[k][lane];
+      acc.x = fadd(acc.x, x.x);
+      acc.y = fadd(acc.y, x.y);
+      acc.z = fadd(acc.z, x.z);
+      acc.w = fadd(acc.w, x.w);
     }
-    __syncthreads();
   }
+  const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+  W* row = gw + (size_t)which.y * a.width;
+#pragma unroll
+  for (int k = 0; k < 4; k++)
+    if (c + k < a.width) {
+      const float r = fmul(v[k], a.scale);
+      row[c + k] = from_f32<W>(a.accumulate ? fadd(to_f32(row[c + k]), r) : r);
+    }
 }
 
 size_t up256(size_t b) { return (b + 255) & ~size_t(255); }
 
 struct Layout {
   unsigned piece, pieces;
-  size_t ld, list, bitmap, crossing, partial, total;
+  size_t ld, list, crossing, partial, total;
 };
-Layout layout_of(size_t n, size_t vocab, size_t width) {
+Layout layout_of(size_t n, size_t width) {
   Layout l;
   size_t piece = kMinPiece;
   while ((n + piece - 1) / piece > kMaxPieces) piece *= 2;
   l.piece = (unsigned)piece;
   l.pieces = (unsigned)((n + piece - 1) / piece);
   l.ld = (width + 3) & ~size_t(3);
-  l.list = up256(n * 4);
-  l.bitmap = up256((vocab + 31) / 32 * 4);
-  l.crossing = up256(((size_t)l.pieces + 1) * 4);
+  l.list = up256(n * 8);
+  l.crossing = up256(((size_t)l.pieces + l.pieces / kLong + 1) * 8);
   l.partial = (size_t)l.pieces * 2 * l.ld * 4;
-  l.total = 4 * l.list + l.bitmap + l.crossing + l.partial;
+  l.total = 256 + 2 * l.list + l.crossing + l.partial;
   return l;
 }
 
@@ -557,13 +674,14 @@ cudaError_t sort_ids(IndexArray ids, unsigned n, size_t vocab, long long padding
   while (total_bits < 32 && (vocab >> total_bits)) total_bits++;
   const int passes = (total_bits + kSortMaxBits - 1) / kSortMaxBits;
   const int bits = (total_bits + passes - 1) / passes;
-  // about 128 keys a warp before another block joins
+  // a key a thread before another block joins
   unsigned blocks = 1;
-  while (blocks < kSortMaxCluster && (size_t)blocks * kSortWarps * 128 < n) blocks *= 2;
+  while (blocks < kSortMaxCluster && blocks * kSortThreads < n) blocks *= 2;
   const size_t smem = (size_t)kSortWarps * (1u << bits) * 4;
-  cudaError_t e = cudaFuncSetAttribute(
-      sort_ids_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-      kSortWarps * (1 << kSortMaxBits) * 4);
+  const size_t per_warp = (n + (size_t)blocks * kSortWarps - 1) / ((size_t)blocks * kSortWarps);
+  const auto kernel = per_warp <= 128 ? sort_ids_kernel<4, true> : sort_ids_kernel<4, false>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       kSortWarps * (1 << kSortMaxBits) * 4);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks);
@@ -578,7 +696,7 @@ cudaError_t sort_ids(IndexArray ids, unsigned n, size_t vocab, long long padding
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   *passes_out = passes;
-  return cudaLaunchKernelEx(&cfg, sort_ids_kernel, ids, n, (long long)vocab, padding, bits, passes,
+  return cudaLaunchKernelEx(&cfg, kernel, ids, n, (long long)vocab, padding, bits, passes,
                             out, bad);
 }
 
@@ -594,7 +712,7 @@ cudaError_t sums_of(const void* g, void* gw, Plan a, cudaStream_t s) {
   if (!a.accumulate) {
     // 128 KB of the table to a block that writes zeros
     const size_t row = a.width * sizeof(W);
-    a.zero_rows = (unsigned)std::max<size_t>(1, std::min<size_t>((size_t)131072 / row, 1u << 20));
+    a.zero_rows = (unsigned)std::max<size_t>(1, std::min<size_t>((size_t)131072 / row, kZeroRows));
     zero_blocks = ((size_t)a.vocab + a.zero_rows - 1) / a.zero_rows;
   }
   if (sum_blocks + zero_blocks > 0x7fffffffull) return cudaErrorInvalidValue;
@@ -604,8 +722,13 @@ cudaError_t sums_of(const void* g, void* gw, Plan a, cudaStream_t s) {
       static_cast<const T*>(g), static_cast<W*>(gw), a);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || a.pieces < 2) return e;
-  join_kernel<W><<<(unsigned)std::min<size_t>((size_t)a.pieces * ((a.width + 127) / 128), 592),
-                   kThreads, 0, s>>>(static_cast<W*>(gw), a);
+  const size_t short_tiles = (a.width + kThreads * 4 - 1) / (kThreads * 4);
+  const size_t long_tiles = (a.width + 127) / 128;
+  const size_t blocks = a.pieces * short_tiles + (a.pieces / kLong + 1) * long_tiles;
+  if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
+  join_kernel<W><<<(unsigned)blocks, kThreads, 0, s>>>(static_cast<W*>(gw), a,
+                                                       (unsigned)short_tiles,
+                                                       (unsigned)long_tiles);
   return cudaGetLastError();
 }
 
@@ -635,8 +758,8 @@ cudaError_t launch_embedding(StoreType t, const void* weight, const void* ids, b
   return cudaErrorInvalidValue;
 }
 
-size_t embedding_backward_scratch(size_t n, size_t vocab, size_t width) {
-  return layout_of(n, vocab, width).total;
+size_t embedding_backward_scratch(size_t n, size_t width) {
+  return layout_of(n, width).total;
 }
 
 cudaError_t launch_embedding_backward(StoreType t, const void* grad_output, const void* ids,
@@ -649,16 +772,14 @@ cudaError_t launch_embedding_backward(StoreType t, const void* grad_output, cons
     return accumulate ? cudaSuccess
                       : cudaMemsetAsync(grad_weight, 0,
                                         vocab * width * (narrow ? store_bytes(t) : 4), s);
-  const Layout l = layout_of(n, vocab, width);
+  const Layout l = layout_of(n, width);
   char* p = static_cast<char*>(scratch);
   Sorted sorted;
-  sorted.key[0] = reinterpret_cast<unsigned*>(p);
-  sorted.key[1] = reinterpret_cast<unsigned*>(p + l.list);
-  sorted.pos[0] = reinterpret_cast<unsigned*>(p + 2 * l.list);
-  sorted.pos[1] = reinterpret_cast<unsigned*>(p + 3 * l.list);
-  p += 4 * l.list;
-  sorted.present = reinterpret_cast<unsigned*>(p);
-  sorted.crossing = reinterpret_cast<unsigned*>(p + l.bitmap);
+  sorted.count = reinterpret_cast<unsigned*>(p);
+  p += 256;
+  sorted.pair[0] = reinterpret_cast<uint2*>(p);
+  sorted.pair[1] = reinterpret_cast<uint2*>(p + l.list);
+  p += 2 * l.list;
   int passes = 0;
   const cudaError_t e = sort_ids(IndexArray{ids, wide}, (unsigned)n, vocab, padding, sorted, bad,
                                  &passes, s);
@@ -667,11 +788,11 @@ cudaError_t launch_embedding_backward(StoreType t, const void* grad_output, cons
   a.n = (unsigned)n;
   a.piece = l.piece;
   a.pieces = l.pieces;
-  a.key = sorted.key[passes & 1];
-  a.pos = sorted.pos[passes & 1];
-  a.present = sorted.present;
-  a.crossing = sorted.crossing;
-  a.partial = reinterpret_cast<float*>(p + l.bitmap + l.crossing);
+  a.pair = sorted.pair[passes & 1];
+  a.count = sorted.count;
+  a.crossing = reinterpret_cast<uint2*>(p);
+  a.crossing_long = a.crossing + l.pieces;
+  a.partial = reinterpret_cast<float*>(p + l.crossing);
   a.ld = l.ld;
   a.vocab = (long long)vocab;
   a.width = width;

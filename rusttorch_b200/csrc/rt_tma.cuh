@@ -95,6 +95,19 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, unsigned b
       : "memory");
 }
 
+// `bytes` (a multiple of 16) from shared `src` to global `dst` (both 16-byte
+// aligned) as one bulk copy; the shared memory may change or go once
+// bulk_store_wait has returned in the thread that stored.
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, unsigned bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+               "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_store_wait() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
 // Orders this thread's earlier generic-proxy accesses of shared memory before
 // later async-proxy (bulk copy) writes to it.
 __device__ __forceinline__ void fence_proxy_async_smem() {
