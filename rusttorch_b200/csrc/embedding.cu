@@ -14,6 +14,7 @@
 //     launch other blocks write the zeros of the ids that do not occur;
 //  3. join_kernel adds up the partial sums.
 // No floating-point atomics: the order of every sum follows from ids alone.
+#include "rt_chain.cuh"
 #include "rt_internal.h"
 #include "rt_libm.cuh"
 #include "rt_tma.cuh"
@@ -248,6 +249,7 @@ sort_ids_kernel(IndexArray ids, unsigned n, long long vocab, long long padding, 
   __shared__ unsigned block_total[1 << kSortMaxBits];    // read by the cluster
   __shared__ unsigned base[1 << kSortMaxBits];           // where the block's digits go
   __shared__ unsigned warp_sum[kSortWarps];
+  let_next_kernel_start();
   cg::cluster_group cluster = cg::this_cluster();
   const unsigned rank = cluster.block_rank(), blocks = cluster.num_blocks();
   const unsigned bins = 1u << bits;
@@ -287,21 +289,26 @@ sort_ids_kernel(IndexArray ids, unsigned n, long long vocab, long long padding, 
     // to[j]: how many of the warp's keys before this one have its digit, on
     // top of what `mine` starts with
     auto rank_keys = [&](unsigned from) {
+      unsigned same[K];                 // the lanes with this one's digit
+#pragma unroll
+      for (int j = 0; j < K; j++) {
+        const unsigned digit = (key[j] >> shift) & (bins - 1);
+        same[j] = __ballot_sync(0xffffffffu, from + j * 32 + lane < end);
+#pragma unroll
+        for (int d = 0; d < kSortMaxBits; d++) {   // bits above `bits` are 0 in every lane
+          const unsigned m = __ballot_sync(0xffffffffu, (digit >> d) & 1u);
+          same[j] &= (digit >> d) & 1u ? m : ~m;
+        }
+      }
 #pragma unroll
       for (int j = 0; j < K; j++) {
         if (from + j * 32 >= end) break;        // the warp's lanes agree
         const bool live = from + j * 32 + lane < end;
         const unsigned digit = (key[j] >> shift) & (bins - 1);
-        unsigned same = __ballot_sync(0xffffffffu, live);
-#pragma unroll
-        for (int d = 0; d < kSortMaxBits; d++) {   // bits above `bits` are 0 in every lane
-          const unsigned m = __ballot_sync(0xffffffffu, (digit >> d) & 1u);
-          same &= (digit >> d) & 1u ? m : ~m;
-        }
-        const unsigned before = __popc(same & ((1u << lane) - 1));
+        const unsigned before = __popc(same[j] & ((1u << lane) - 1));
         if (live) to[j] = mine[digit] + before;
         __syncwarp();
-        if (live && before == 0) mine[digit] += __popc(same);
+        if (live && before == 0) mine[digit] += __popc(same[j]);
         __syncwarp();
       }
     };
@@ -490,7 +497,9 @@ template <class T, class W, int VW>
 __global__ void __launch_bounds__(kThreads)
 segment_kernel(const T* g, W* gw, Plan a) {
   constexpr int N = Row<T>::N;
-  constexpr int U = VW * sizeof(T) >= 8 ? 8 : 4;
+  constexpr int U = VW * sizeof(T) >= 8 ? 4 : 2;
+  wait_for_previous_kernel();   // the sorted list
+  let_next_kernel_start();
   if (blockIdx.x >= a.sum_blocks) {
     write_zeros(a, gw);
     return;
@@ -591,6 +600,7 @@ template <class W>
 __global__ void __launch_bounds__(kThreads)
 join_kernel(W* gw, Plan a, unsigned short_tiles, unsigned long_tiles) {
   __shared__ float4 eighth[8][32];
+  wait_for_previous_kernel();   // the partial sums
   const unsigned part = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned longs = (a.pieces / kLong + 1) * long_tiles;
   const bool is_long = blockIdx.x < longs;
@@ -718,18 +728,16 @@ cudaError_t sums_of(const void* g, void* gw, Plan a, cudaStream_t s) {
   if (sum_blocks + zero_blocks > 0x7fffffffull) return cudaErrorInvalidValue;
   a.sum_blocks = (unsigned)sum_blocks;
   const size_t smem = (size_t)a.per_block * 2 * kSub * 4;
-  segment_kernel<T, W, VW><<<(unsigned)(sum_blocks + zero_blocks), kThreads, smem, s>>>(
-      static_cast<const T*>(g), static_cast<W*>(gw), a);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = launch_after(segment_kernel<T, W, VW>, (unsigned)(sum_blocks + zero_blocks),
+                               kThreads, smem, s, static_cast<const T*>(g), static_cast<W*>(gw),
+                               a);
   if (e != cudaSuccess || a.pieces < 2) return e;
   const size_t short_tiles = (a.width + kThreads * 4 - 1) / (kThreads * 4);
   const size_t long_tiles = (a.width + 127) / 128;
   const size_t blocks = a.pieces * short_tiles + (a.pieces / kLong + 1) * long_tiles;
   if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
-  join_kernel<W><<<(unsigned)blocks, kThreads, 0, s>>>(static_cast<W*>(gw), a,
-                                                       (unsigned)short_tiles,
-                                                       (unsigned)long_tiles);
-  return cudaGetLastError();
+  return launch_after(join_kernel<W>, (unsigned)blocks, kThreads, 0, s, static_cast<W*>(gw), a,
+                      (unsigned)short_tiles, (unsigned)long_tiles);
 }
 
 template <class T, class W>
