@@ -179,7 +179,7 @@ rtc_result check_loss(const rtc_tensor* logits, const rtc_tensor* targets, int64
   a->vocab = vocab;
   a->ignore = ignore_index;
   a->reduction = reduction;
-  a->bad = nullptr;
+  a->bad = a->gave_up = nullptr;
   return ok();
 }
 
@@ -236,6 +236,7 @@ extern "C" rtc_result rtc_softmax_cross_entropy(const rtc_tensor* logits,
   if (a.rows == 0 && reduction == RTC_REDUCE_NONE) return ok();
   return on_device(logits->device, token_loss_scratch(a), ctx, [&](void* scratch, int* bad) {
     a.bad = bad;
+    a.gave_up = wait_timeout_flag(logits->device);
     return launch_token_loss(a, f(loss), stats ? f(stats) : nullptr, scratch, thread_stream());
   });
 }
@@ -255,6 +256,7 @@ extern "C" rtc_result rtc_softmax_cross_entropy_backward(
   if (a.rows == 0) return ok();
   return on_device(logits->device, token_loss_scratch(a), ctx, [&](void* scratch, int* bad) {
     a.bad = bad;
+    a.gave_up = wait_timeout_flag(logits->device);
     return launch_token_loss_backward(a, cf(grad_output), cf(stats), grad_logits->data, scratch,
                                       thread_stream());
   });
@@ -277,6 +279,7 @@ extern "C" rtc_result rtc_softmax_cross_entropy_grad(const rtc_tensor* logits,
   if (a.rows == 0 && reduction == RTC_REDUCE_NONE) return ok();
   return on_device(logits->device, token_loss_scratch(a), ctx, [&](void* scratch, int* bad) {
     a.bad = bad;
+    a.gave_up = wait_timeout_flag(logits->device);
     return launch_token_loss_grad(a, grad_scale, f(loss), grad_logits->data, scratch,
                                   thread_stream());
   });

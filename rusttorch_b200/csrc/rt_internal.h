@@ -219,7 +219,8 @@ struct TokenLoss {
   size_t rows, vocab;
   long long ignore;
   int reduction;         // RTC_REDUCE_*
-  int* bad;
+  int* bad;              // the device's flags: a target outside the vocabulary,
+  int* gave_up;          // a wait that ran out
 };
 // Scratch of the calls below, 256-byte aligned.
 size_t token_loss_scratch(const TokenLoss& a);

@@ -108,6 +108,26 @@ __device__ __forceinline__ void bulk_store_wait() {
   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
+// A cluster barrier in two halves; the arrival orders no memory access.
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Stores a float2 into block `rank` of this cluster, at the place that `dst`
+// has in this block, and counts its 8 bytes at that block's mbarrier `bar`.
+__device__ __forceinline__ void store_async(float2* dst, float2 v, uint64_t* bar, unsigned rank) {
+  uint32_t d, b;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_u32(dst)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(smem_u32(bar)), "r"(rank));
+  asm volatile(
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(d),
+      "f"(v.x), "f"(v.y), "r"(b)
+      : "memory");
+}
+
 // Orders this thread's earlier generic-proxy accesses of shared memory before
 // later async-proxy (bulk copy) writes to it.
 __device__ __forceinline__ void fence_proxy_async_smem() {

@@ -1,0 +1,58 @@
+// token_loss.h — what the token loss's kernels (token_loss.cuh, one file per
+// storage type) and its launchers (token_loss.cu) share.
+#pragma once
+#include "rt_internal.h"
+#include "rt_types.cuh"
+
+namespace rt {
+
+// How many rows count, at least 1 (a mean over none is 0), and its inverse.
+struct Count {
+  unsigned long long rows;
+  float inverse;
+};
+
+struct LossArgs {
+  IndexArray targets;
+  size_t rows;
+  unsigned vocab;
+  long long ignore;
+  float* row_losses;                   // [rows of the call]
+  float* stats;                        // null, or [rows, 3]
+  void* grad;                          // null, or the gradient
+  float grad_scale;
+  const Count* count;                  // null, or what a mean divides by
+  int* bad;
+  int* gave_up;                        // the flag of a wait that ran out
+  bool alike;                          // grad's rows start where logits' do, modulo 16 bytes
+};
+
+// Statistics and losses of every row, and the gradient unless it is null and
+// the rows fit on chip.
+#define RT_TOKEN_LOSS_DECL(NAME)                                                                \
+  cudaError_t token_rows_##NAME(const TokenLoss& t, const LossArgs& a, bool chained,            \
+                                cudaStream_t s);                                                \
+  cudaError_t token_grad_##NAME(const TokenLoss& t, const float* stats, const float* upstream,  \
+                                float grad_scale, const Count* count, void* grad, bool chained, \
+                                cudaStream_t s);
+RT_TOKEN_LOSS_DECL(f32)
+RT_TOKEN_LOSS_DECL(bf16)
+RT_TOKEN_LOSS_DECL(f16)
+#undef RT_TOKEN_LOSS_DECL
+
+constexpr size_t kMaxGrid = 0x7fffffff;
+constexpr int kMaxCluster = 8;        // blocks to a row
+// 16-byte vectors of a row that a block holds: two buffers of them in each of
+// per_sm blocks fill an SM's shared memory (less 1 KB and the tables of each).
+__host__ __device__ constexpr unsigned run_vecs(int per_sm) {
+  return per_sm == 16 ? 400 : per_sm == 8 ? 840 : 6912 / per_sm;
+}
+
+// The vectors that a row may have.
+inline size_t vecs_of(const TokenLoss& a) { return (a.vocab * store_bytes(a.type) + 15) / 16; }
+// Whether a row fits on chip, so that one pass gives its gradient too.
+inline bool fits_cluster(const TokenLoss& a) {
+  return vecs_of(a) <= kMaxCluster * run_vecs(1);
+}
+
+}  // namespace rt
