@@ -340,6 +340,78 @@ rtc_result check_moments(const rtc_tensor* p, const rtc_tensor* codes, const rtc
 
 }  // namespace
 
+namespace {
+
+// Tensor i of the lists, with the errors that its checks give.
+rtc_result check_listed(const rtc_tensor* params, const rtc_tensor* grads, const rtc_tensor* m,
+                        const rtc_tensor* v, const rtc_tensor* m_scales,
+                        const rtc_tensor* v_scales, const rtc_tensor* copies, size_t i) {
+  const rtc_tensor* p = &params[i];
+  TRY(check_token_desc(p, of("params", i).c_str()));
+  TRY(check_token_desc(&grads[i], of("grads", i).c_str()));
+  TRY(check_token_desc(&m[i], of("m", i).c_str()));
+  TRY(check_token_desc(&v[i], of("v", i).c_str()));
+  StoreType type;
+  TRY(need_dtype(p, RTC_F32, of("params", i)));
+  TRY(need_float(&grads[i], of("grads", i), &type));
+  if (!same_shape(p, &grads[i])) return shape_mismatch(of("grads", i), p, &grads[i]);
+  if (!same_shape(p, &m[i])) return shape_mismatch(of("m", i), p, &m[i]);
+  if (!same_shape(p, &v[i])) return shape_mismatch(of("v", i), p, &v[i]);
+  TRY(one_device(&params[0], p));
+  TRY(one_device(p, &grads[i]));
+  TRY(one_device(p, &m[i]));
+  TRY(one_device(p, &v[i]));
+  if (m_scales) {
+    TRY(check_moments(p, &m[i], &m_scales[i], of("m", i), of("m_scales", i)));
+    TRY(check_moments(p, &v[i], &v_scales[i], of("v", i), of("v_scales", i)));
+  } else {
+    TRY(need_dtype(&m[i], RTC_F32, of("m", i)));
+    TRY(need_dtype(&v[i], RTC_F32, of("v", i)));
+  }
+  if (copies) {
+    TRY(check_token_desc(&copies[i], of("copies", i).c_str()));
+    if (copies[i].dtype != RTC_BF16 && copies[i].dtype != RTC_F16)
+      return dtype_mismatch(of("copies", i), "bfloat16 or float16", dtype_display(copies[i].dtype));
+    if (!same_shape(p, &copies[i])) return shape_mismatch(of("copies", i), p, &copies[i]);
+    TRY(one_device(p, &copies[i]));
+  }
+  return ok();
+}
+
+// Whether a tensor passes check_listed as most do: contiguous without strides,
+// on p's device, of the type and shape that its list wants.  A short-cut:
+// what it does not know goes to check_listed.
+bool plain(const rtc_tensor* t) {
+  if (t->strides || t->device < 0 || (t->ndim > 0 && !t->shape)) return false;
+  unsigned __int128 prod = 1;
+  for (size_t i = 0; i < t->ndim; i++) {
+    prod *= t->shape[i];
+    if (prod > SIZE_MAX) return false;
+  }
+  return prod == t->numel && (t->numel == 0 || t->data) &&
+         reinterpret_cast<uintptr_t>(t->data) % dtype_bytes(t->dtype) == 0;
+}
+bool plain_f32(const rtc_tensor* t) { return t->dtype == RTC_F32 && plain(t); }
+bool plain_like(const rtc_tensor* t, const rtc_tensor* p) {
+  return plain(t) && t->device == p->device && same_shape(t, p);
+}
+bool plain_moment(const rtc_tensor* t, const rtc_tensor* p, bool eight) {
+  return t->dtype == (eight ? RTC_F8E4M3 : RTC_F32) && plain_like(t, p);
+}
+bool plain_grad(const rtc_tensor* t, const rtc_tensor* p) {
+  StoreType type;
+  return store_type(t->dtype, &type) && plain_like(t, p);
+}
+bool plain_copy(const rtc_tensor* t, const rtc_tensor* p) {
+  return (t->dtype == RTC_BF16 || t->dtype == RTC_F16) && plain_like(t, p);
+}
+bool plain_scales(const rtc_tensor* t, const rtc_tensor* p) {
+  return t->dtype == RTC_F32 && plain(t) && t->device == p->device &&
+         t->numel == (p->numel + kMomentBlock - 1) / kMomentBlock;
+}
+
+}  // namespace
+
 extern "C" rtc_result rtc_adamw_update_multi(
     const rtc_tensor* params, const rtc_tensor* grads, const rtc_tensor* m, const rtc_tensor* v,
     const rtc_tensor* m_scales, const rtc_tensor* v_scales, const rtc_tensor* copies, size_t n,
@@ -363,39 +435,19 @@ extern "C" rtc_result rtc_adamw_update_multi(
   ranges.reserve(7 * n);
   for (size_t i = 0; i < n; i++) {
     const rtc_tensor* p = &params[i];
-    TRY(check_token_desc(p, of("params", i).c_str()));
-    TRY(check_token_desc(&grads[i], of("grads", i).c_str()));
-    TRY(check_token_desc(&m[i], of("m", i).c_str()));
-    TRY(check_token_desc(&v[i], of("v", i).c_str()));
     AdamTensor& t = list[i];
-    TRY(need_dtype(p, RTC_F32, of("params", i)));
-    TRY(need_float(&grads[i], of("grads", i), &t.gtype));
-    if (!same_shape(p, &grads[i])) return shape_mismatch(of("grads", i), p, &grads[i]);
-    if (!same_shape(p, &m[i])) return shape_mismatch(of("m", i), p, &m[i]);
-    if (!same_shape(p, &v[i])) return shape_mismatch(of("v", i), p, &v[i]);
-    TRY(one_device(&params[0], p));
-    TRY(one_device(p, &grads[i]));
-    TRY(one_device(p, &m[i]));
-    TRY(one_device(p, &v[i]));
-    t.ms = t.vs = nullptr;
-    if (eight) {
-      TRY(check_moments(p, &m[i], &m_scales[i], of("m", i), of("m_scales", i)));
-      TRY(check_moments(p, &v[i], &v_scales[i], of("v", i), of("v_scales", i)));
-      t.ms = f(&m_scales[i]);
-      t.vs = f(&v_scales[i]);
-    } else {
-      TRY(need_dtype(&m[i], RTC_F32, of("m", i)));
-      TRY(need_dtype(&v[i], RTC_F32, of("v", i)));
-    }
+    // what is right is not named: the names are built for an error alone
+    const bool plain = plain_f32(p) && plain_moment(&m[i], p, eight) && plain_moment(&v[i], p, eight) &&
+                       plain_grad(&grads[i], p) &&
+                       (!eight || (plain_scales(&m_scales[i], p) && plain_scales(&v_scales[i], p))) &&
+                       (!copies || plain_copy(&copies[i], p)) && p->device == params[0].device;
+    if (!plain) TRY(check_listed(params, grads, m, v, m_scales, v_scales, copies, i));
+    store_type(grads[i].dtype, &t.gtype);
+    t.ms = eight ? f(&m_scales[i]) : nullptr;
+    t.vs = eight ? f(&v_scales[i]) : nullptr;
     t.copy = nullptr;
     t.ctype = kBF16;
     if (copies) {
-      TRY(check_token_desc(&copies[i], of("copies", i).c_str()));
-      if (copies[i].dtype != RTC_BF16 && copies[i].dtype != RTC_F16)
-        return dtype_mismatch(of("copies", i), "bfloat16 or float16",
-                              dtype_display(copies[i].dtype));
-      if (!same_shape(p, &copies[i])) return shape_mismatch(of("copies", i), p, &copies[i]);
-      TRY(one_device(p, &copies[i]));
       store_type(copies[i].dtype, &t.ctype);
       t.copy = copies[i].data;
     }
