@@ -546,7 +546,7 @@ rtc_result rtc_softmax_cross_entropy_grad(const rtc_tensor* logits, const rtc_te
  *    sqrt(v).  Each step decodes, updates in f32
  *      m' = m*b1 + g*(1-b1), v' = v*b2 + (g*g)*(1-b2), r = sqrt(v'),
  *      p' = p - (m'/(r*c2 + eps))*(lr/(1-b1^t)) - p*(lr*wd),
- *      c2 = 1/sqrt(1-b2^t),
+ *      c2 = 1/sqrt(1-b2^t), the quotient within 2 ulp, eps at least 2^-126,
  *    and encodes m' and r with stochastic rounding, so that averages move even
  *    where one step changes them by less than a code's width: the random bits
  *    are a function of (seed, i, element) alone.  A non-zero r never becomes 0;

@@ -478,11 +478,12 @@ extern "C" rtc_result rtc_adamw_update_multi(
     c8.b2 = c.b2;
     c8.one_minus_b2 = c.one_minus_b2;
     c8.c2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)timestep)));
-    c8.eps = c.eps;
+    c8.eps = std::max(c.eps, 0x1p-126f);   // a normal number, for the reciprocal
     c8.step = (float)(learning_rate / (1.0 - std::pow(beta1, (double)timestep)));
-    c8.lr_wd = c.lr_wd;
-    c8.decay = c.decay;
-    return launch_adam8_multi(list.data(), n, c8, seed, thread_stream());
+    c8.lr_wd = c.decay ? c.lr_wd : 0.0f;
+    c8.one = 1.0f;
+    return launch_adam8_multi(list.data(), n, c8, seed, wait_timeout_flag(params[0].device),
+                              thread_stream());
   });
 }
 

@@ -251,12 +251,13 @@ constexpr int kMomentBlock = 128;
 // Coefficients of a step with 8-bit moments.
 struct Adam8Coeffs {
   float b1, one_minus_b1, b2, one_minus_b2, c2, eps, step;
-  float lr_wd;
-  int decay;
+  float lr_wd;             // 0 without decay
+  float one;               // 1 (f2_add)
 };
 cudaError_t launch_adam_multi(const AdamTensor* t, size_t n, const AdamCoeffs& c, cudaStream_t s);
+// gave_up: the device flag of a wait that ran out.
 cudaError_t launch_adam8_multi(const AdamTensor* t, size_t n, const Adam8Coeffs& c, uint64_t seed,
-                               cudaStream_t s);
+                               int* gave_up, cudaStream_t s);
 cudaError_t launch_adam8_pack(const float* m, const float* v, void* mc, float* ms, void* vc,
                               float* vs, size_t n, cudaStream_t s);
 cudaError_t launch_adam8_unpack(const void* mc, const float* ms, const void* vc, const float* vs,

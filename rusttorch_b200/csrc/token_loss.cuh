@@ -19,6 +19,7 @@
 #include "rt_chain.cuh"
 #include "rt_internal.h"
 #include "rt_libm.cuh"
+#include "rt_pairs.cuh"
 #include "rt_tma.cuh"
 #include "rt_types.cuh"
 #include "token_loss.h"
@@ -73,34 +74,6 @@ __device__ __forceinline__ float exp_below(float x, float m) {
   return exp2_approx(fmul(fsub(x, m), kLog2e));
 }
 
-// Two f32 in a 64-bit register: one instruction rounds both results.
-struct F2 {
-  uint64_t v;
-};
-__device__ __forceinline__ F2 f2_of(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void f2_to(F2 x, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
-}
-__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-
 // e^(x - m) of pairs, m >= x, as 2^(x L - m L) for L = log2 e rounded to f32:
 // m L as `hi`, its f32 value, and the factor 2^lo of what that leaves, so the
 // product x L and the difference round once together, and the result times
@@ -125,7 +98,7 @@ __device__ __forceinline__ Under under(float m) {
 template <bool WIDE>
 __device__ __forceinline__ F2 term2(F2 x, const Under& u) {
   F2 y;
-  if constexpr (WIDE) y = f2_mul(f2_add(x, f2_of(-u.m, -u.m)), f2_of(kLog2e, kLog2e));
+  if constexpr (WIDE) y = f2_mul(f2_sum(x, f2_of(-u.m, -u.m)), f2_of(kLog2e, kLog2e));
   else y = f2_fma(x, f2_of(kLog2e, kLog2e), u.hi);
   float a, b;
   f2_to(y, a, b);
@@ -217,7 +190,7 @@ __device__ __forceinline__ void drop(Vec<T>& v, int e) {
 template <bool WIDE, class T>
 __device__ __forceinline__ void add_terms(const Vec<T>& v, const Under& u, F2& s) {
 #pragma unroll
-  for (int i = 0; i < Vec<T>::N / 2; i++) s = f2_add(s, term2<WIDE>(pair_of(v, i), u));
+  for (int i = 0; i < Vec<T>::N / 2; i++) s = f2_sum(s, term2<WIDE>(pair_of(v, i), u));
 }
 // v's terms times k (which holds the factor).
 template <bool WIDE, class T>

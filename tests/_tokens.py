@@ -207,7 +207,12 @@ def decode(codes, scales):
 
 
 def adamw8(p, g, mc, ms, vc, vs, lr, b1, b2, eps, wd, t, seed, index):
-    """One step with 8-bit moments, every operation rounded to f32 as documented."""
+    """One step with 8-bit moments, every operation rounded to f32 as documented:
+    (parameters, largest error of theirs, codes and scales).  The quotient is
+    within 2 ulp (2^-22 of it) of the rounded one here, which its product with
+    the step size passes on with a rounding of its own (2^-23 covers both
+    sides'), and each of the two differences rounds at most half an ulp apart
+    from a value that close: 2^-23 of the parameter each."""
     p, g = np.asarray(p, F32), np.asarray(g, F32)
     with np.errstate(all="ignore"):
         m, root = decode(mc, ms), decode(vc, vs)
@@ -216,7 +221,8 @@ def adamw8(p, g, mc, ms, vc, vs, lr, b1, b2, eps, wd, t, seed, index):
         v = (root * root) * fb2 + (g * g) * (F32(1) - fb2)
         r = np.sqrt(v)
         den = r * F32(1 / np.sqrt(1 - b2 ** t)) + F32(eps)
-        out = p - (m / den) * F32(lr / (1 - b1 ** t))
+        move = (m / den) * F32(lr / (1 - b1 ** t))
+        out = p - move
         if wd > 0:
             out = out - p * F32(lr * wd)
     i = np.arange(len(p), dtype=np.uint64)
@@ -225,4 +231,6 @@ def adamw8(p, g, mc, ms, vc, vs, lr, b1, b2, eps, wd, t, seed, index):
     mc, ms = encode(m, bits & np.uint32(0xffff), False)
     vc, vs = encode(r, bits >> np.uint32(16), True)
     assert out.dtype == F32
-    return out, mc, ms, vc, vs
+    with np.errstate(invalid="ignore"):
+        bound = np.abs(move.astype(np.float64)) * (2.0 ** -22 + 2.0 ** -23) + (np.abs(p) + np.abs(out)).astype(np.float64) * 2.0 ** -23
+    return out, bound, mc, ms, vc, vs

@@ -306,7 +306,7 @@ def test_average_follows_its_input_in_8_bits():
     vc, vs = K.encode(np.full(n, 1.0, np.float32), None, True)
     p, g = np.zeros(n, np.float32), np.full(n, 0.1, np.float32)
     for t in range(1, 1001):
-        p, mc, ms, vc, vs = K.adamw8(p, g, mc, ms, vc, vs, 1e-3, 0.9, b2, 1e-8, 0.0, t, t, 0)
+        p, _, mc, ms, vc, vs = K.adamw8(p, g, mc, ms, vc, vs, 1e-3, 0.9, b2, 1e-8, 0.0, t, t, 0)
     root = K.decode(vc, vs).astype(np.float64)
     assert abs(root.mean() / np.sqrt(0.01 * (1 + 99 * b2 ** 1000)) - 1) < 0.05
 

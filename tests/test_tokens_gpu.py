@@ -40,7 +40,8 @@ def shifted(rt, a, dtype, elements, keep=[]):
 def same(got, want):
     got, want = np.asarray(got, np.float32), np.asarray(want, np.float32)
     assert got.shape == want.shape
-    assert ((got.view(np.uint32) == want.view(np.uint32)) | (np.isnan(got) & np.isnan(want))).all()
+    off = (got.view(np.uint32) != want.view(np.uint32)) & ~(np.isnan(got) & np.isnan(want))
+    assert not off.any(), (int(off.sum()), np.argwhere(off)[:3].tolist(), got[off][:3], want[off][:3])
 
 
 def near(got, want, bound):
@@ -493,7 +494,8 @@ def eight(rt, host):
 
 @pytest.mark.parametrize("gtype", DTYPES)
 def test_adamw_multi_in_8_bits(rt, gtype):
-    """Every operation is one IEEE rounding, so three steps agree bit for bit."""
+    """Every operation that leads to the codes is one IEEE rounding, so three
+    steps' moments agree bit for bit; the parameters within the quotient's 2 ulp."""
     rng = np.random.default_rng(14)
     host = [adam_state(rng, s, gtype) for s in SIZES]
     host[4][3][100:400] *= 1e-12          # blocks of small and of widely spread moments
@@ -510,9 +512,10 @@ def test_adamw_multi_in_8_bits(rt, gtype):
         rt.adamw_update_multi(P, G, [d[0] for d in dev8], [d[2] for d in dev8], *HYPER, t, m_scales=[d[1] for d in dev8],
                               v_scales=[d[3] for d in dev8], copies=copies, seed=t * 10 ** 12)
         for i, h in enumerate(host):
-            p, *codes = K.adamw8(h[0].ravel(), h[1].ravel(), *host8[i], *HYPER, t, t * 10 ** 12, i)
-            h[0], host8[i] = p.reshape(h[0].shape), codes
-            same(P[i].to_numpy(), h[0])
+            p, bound, *codes = K.adamw8(h[0].ravel(), h[1].ravel(), *host8[i], *HYPER, t, t * 10 ** 12, i)
+            host8[i] = codes
+            h[0] = P[i].to_numpy()
+            near(h[0].ravel(), p, bound)
             same(get(copies[i]), K.bf16(h[0]))
             for d, w in zip(dev8[i], codes):
                 assert (d.to_numpy().ravel() == w).all()
@@ -525,8 +528,8 @@ def test_adamw_multi_in_8_bits_of_values_that_are_not_finite(rt):
     dev, codes = eight(rt, h)
     P, G = put(rt, h[0]), put(rt, h[1])
     rt.adamw_update_multi([P], [G], [dev[0]], [dev[2]], *HYPER, 1, m_scales=[dev[1]], v_scales=[dev[3]], seed=5)
-    p, *want = K.adamw8(h[0], h[1], *codes, *HYPER, 1, 5, 0)
-    same(P.to_numpy(), p)
+    p, bound, *want = K.adamw8(h[0], h[1], *codes, *HYPER, 1, 5, 0)
+    near(P.to_numpy(), p, np.nan_to_num(bound))
     for d, w in zip(dev, want):
         assert (d.to_numpy() == w).all()
     v = K.decode(dev[2].to_numpy(), dev[3].to_numpy())
