@@ -84,7 +84,10 @@ __device__ __forceinline__ void store_row(G_* row, size_t first, unsigned G, siz
         Chunk<G_, SW> o;
 #pragma unroll
         for (int e = 0; e < SW; e++) o.x[e] = from_f32<G_>(v[k * VW + h * SW + e]);
-        *reinterpret_cast<Chunk<G_, SW>*>(row + c + h * SW) = o;
+        if constexpr (SW * sizeof(G_) == 16)
+          __stcs(reinterpret_cast<uint4*>(row + c + h * SW), *reinterpret_cast<const uint4*>(&o));
+        else
+          *reinterpret_cast<Chunk<G_, SW>*>(row + c + h * SW) = o;
       }
     }
   }
@@ -214,6 +217,12 @@ constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortMaxCluster = 8;
 constexpr int kSortMaxBits = 9;
 
+// Bytes of the gradient that other blocks zero while one cluster sorts.
+struct Shadow {
+  char* begin;
+  size_t bytes;          // a multiple of 2, as begin is
+};
+
 struct Sorted {
   uint2* pair[2];       // [n] each: key, and where in ids it was; sorted in pair[passes & 1]
   unsigned* count;      // [2]: of the sums that cross pieces, zeroed here
@@ -229,6 +238,33 @@ __device__ __forceinline__ unsigned key_of(const IndexArray& ids, size_t i, long
   return id == padding ? (unsigned)vocab : (unsigned)id;
 }
 
+constexpr unsigned kShadowBytes = 16384;   // zeros that they copy at a time
+
+// `block` of `blocks`, a warp's first lane at a time: the 16-byte-aligned inside
+// by bulk copies of shared zeros, the ends two bytes at a time.
+__device__ __forceinline__ void write_shadow(const Shadow& z, uint4* zeros, unsigned block,
+                                             unsigned blocks) {
+  for (unsigned i = threadIdx.x; i < kShadowBytes / 16; i += kSortThreads)
+    zeros[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  __syncthreads();
+  char* end = z.begin + z.bytes;
+  char* a0 = z.begin + (-reinterpret_cast<intptr_t>(z.begin) & 15);
+  char* a1 = end - (reinterpret_cast<intptr_t>(end) & 15);
+  if (a0 > a1) a0 = a1 = end;
+  if (block == 0 && threadIdx.x < 16) {
+    uint16_t* h = reinterpret_cast<uint16_t*>(threadIdx.x < 8 ? z.begin : a1) + threadIdx.x % 8;
+    if (reinterpret_cast<char*>(h) < (threadIdx.x < 8 ? a0 : end)) *h = 0;
+  }
+  if ((threadIdx.x & 31) == 0) {
+    const size_t step = (size_t)blocks * kSortWarps * kShadowBytes;
+    for (char* q = a0 + ((size_t)block * kSortWarps + (threadIdx.x >> 5)) * kShadowBytes; q < a1;
+         q += step)
+      bulk_store(q, zeros, (unsigned)min((ptrdiff_t)kShadowBytes, (ptrdiff_t)(a1 - q)));
+    bulk_store_done();
+  }
+}
+
 // Stable least-significant-digit radix sort of n keys below 2^(bits * passes)
 // by one cluster.  Every warp owns a contiguous range of the list.  A pass
 // ranks each key among its warp's keys of the same digit (ballots over the
@@ -241,17 +277,22 @@ __device__ __forceinline__ unsigned key_of(const IndexArray& ids, size_t i, long
 // lane, so key and position travel as one, over all the blocks of a cluster.
 // Ids that have no row (outside the vocabulary, or padding) get key = vocab,
 // which sorts last.
+// The grid's further clusters write zeros (Shadow) meanwhile.
 template <int K, bool HELD>
 __global__ void __launch_bounds__(kSortThreads)
 sort_ids_kernel(IndexArray ids, unsigned n, long long vocab, long long padding, int bits,
-                int passes, Sorted out, int* bad) {
-  extern __shared__ unsigned hist[];                     // [kSortWarps][bins]
+                int passes, Sorted out, Shadow shadow, int* bad) {
+  extern __shared__ __align__(16) unsigned hist[];       // [kSortWarps][bins]
   __shared__ unsigned block_total[1 << kSortMaxBits];    // read by the cluster
   __shared__ unsigned base[1 << kSortMaxBits];           // where the block's digits go
   __shared__ unsigned warp_sum[kSortWarps];
   let_next_kernel_start();
   cg::cluster_group cluster = cg::this_cluster();
   const unsigned rank = cluster.block_rank(), blocks = cluster.num_blocks();
+  if (blockIdx.x >= blocks) {
+    write_shadow(shadow, reinterpret_cast<uint4*>(hist), blockIdx.x - blocks, gridDim.x - blocks);
+    return;
+  }
   const unsigned bins = 1u << bits;
   const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned warps = blocks * kSortWarps;
@@ -405,6 +446,7 @@ struct Plan {
   unsigned G, tiles, per_block;
   unsigned sum_blocks;    // then blocks that write zeros
   unsigned zero_rows;     // rows of the table for each of those
+  long long zeroed;       // rows that have their zeros already
 };
 
 __device__ __forceinline__ void prefetch_l2(const void* p) {
@@ -446,7 +488,7 @@ __device__ __forceinline__ void write_zeros(const Plan& a, W* gw) {
   __shared__ unsigned range[2];
   __shared__ uint4 zeros[kZeroBytes / 16];
   for (int i = threadIdx.x; i < kZeroBytes / 16; i += kThreads) zeros[i] = make_uint4(0, 0, 0, 0);
-  const long long v0 = (long long)(blockIdx.x - a.sum_blocks) * a.zero_rows;
+  const long long v0 = a.zeroed + (long long)(blockIdx.x - a.sum_blocks) * a.zero_rows;
   const int rows = (int)min((long long)a.zero_rows, a.vocab - v0);
   if (threadIdx.x < kZeroRows / 32) here[threadIdx.x] = 0;
   if (threadIdx.x < 64) {
@@ -679,7 +721,8 @@ Layout layout_of(size_t n, size_t width) {
 }
 
 cudaError_t sort_ids(IndexArray ids, unsigned n, size_t vocab, long long padding,
-                     const Sorted& out, int* bad, int* passes_out, cudaStream_t s) {
+                     const Sorted& out, const Shadow& shadow, int* bad, int* passes_out,
+                     cudaStream_t s) {
   int total_bits = 1;
   while (total_bits < 32 && (vocab >> total_bits)) total_bits++;
   const int passes = (total_bits + kSortMaxBits - 1) / kSortMaxBits;
@@ -687,14 +730,21 @@ cudaError_t sort_ids(IndexArray ids, unsigned n, size_t vocab, long long padding
   // a key a thread before another block joins
   unsigned blocks = 1;
   while (blocks < kSortMaxCluster && blocks * kSortThreads < n) blocks *= 2;
-  const size_t smem = (size_t)kSortWarps * (1u << bits) * 4;
+  const size_t smem = std::max<size_t>((size_t)kSortWarps * (1u << bits) * 4, kShadowBytes);
   const size_t per_warp = (n + (size_t)blocks * kSortWarps - 1) / ((size_t)blocks * kSortWarps);
   const auto kernel = per_warp <= 128 ? sort_ids_kernel<4, true> : sort_ids_kernel<4, false>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        kSortWarps * (1 << kSortMaxBits) * 4);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks);
+  unsigned others = 0;       // whole clusters, an SM to a block
+  if (shadow.bytes) {
+    int device = 0;
+    cudaGetDevice(&device);
+    const unsigned sms = (unsigned)sm_count(device);
+    others = sms > 2 * blocks ? (sms - blocks) / blocks * blocks : blocks;
+  }
+  cfg.gridDim = dim3(blocks + others);
   cfg.blockDim = dim3(kSortThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -707,7 +757,7 @@ cudaError_t sort_ids(IndexArray ids, unsigned n, size_t vocab, long long padding
   cfg.numAttrs = 1;
   *passes_out = passes;
   return cudaLaunchKernelEx(&cfg, kernel, ids, n, (long long)vocab, padding, bits, passes,
-                            out, bad);
+                            out, shadow, bad);
 }
 
 template <class T, class W, int VW>
@@ -723,7 +773,7 @@ cudaError_t sums_of(const void* g, void* gw, Plan a, cudaStream_t s) {
     // 128 KB of the table to a block that writes zeros
     const size_t row = a.width * sizeof(W);
     a.zero_rows = (unsigned)std::max<size_t>(1, std::min<size_t>((size_t)131072 / row, kZeroRows));
-    zero_blocks = ((size_t)a.vocab + a.zero_rows - 1) / a.zero_rows;
+    zero_blocks = ((size_t)(a.vocab - a.zeroed) + a.zero_rows - 1) / a.zero_rows;
   }
   if (sum_blocks + zero_blocks > 0x7fffffffull) return cudaErrorInvalidValue;
   a.sum_blocks = (unsigned)sum_blocks;
@@ -788,9 +838,20 @@ cudaError_t launch_embedding_backward(StoreType t, const void* grad_output, cons
   sorted.pair[0] = reinterpret_cast<uint2*>(p);
   sorted.pair[1] = reinterpret_cast<uint2*>(p + l.list);
   p += 2 * l.list;
+  // What the other SMs can zero while one cluster sorts, which takes about 8 us
+  // and 0.4 us for each 1000 ids.  Rows with tokens among it are written again,
+  // which costs less than the wait (16384 x 1024 f32 into 50257 rows: 64 us for
+  // 71).
+  const size_t row = width * (narrow ? store_bytes(t) : 4);
+  size_t zeroed = 0;
+  Shadow shadow = {static_cast<char*>(grad_weight), 0};
+  if (!accumulate) {
+    zeroed = std::min(vocab, (((size_t)48 << 20) + std::min<size_t>(n, 32768) * 2048) / row);
+    shadow.bytes = zeroed * row;
+  }
   int passes = 0;
-  const cudaError_t e = sort_ids(IndexArray{ids, wide}, (unsigned)n, vocab, padding, sorted, bad,
-                                 &passes, s);
+  const cudaError_t e = sort_ids(IndexArray{ids, wide}, (unsigned)n, vocab, padding, sorted,
+                                 shadow, bad, &passes, s);
   if (e != cudaSuccess) return e;
   Plan a = {};
   a.n = (unsigned)n;
@@ -806,6 +867,7 @@ cudaError_t launch_embedding_backward(StoreType t, const void* grad_output, cons
   a.width = width;
   a.scale = scale;
   a.accumulate = accumulate;
+  a.zeroed = (long long)zeroed;
   switch (t) {
     case kF32: return sums_any<float, float>(grad_output, grad_weight, a, s);
     case kBF16:

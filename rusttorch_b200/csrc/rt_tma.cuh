@@ -108,6 +108,12 @@ __device__ __forceinline__ void bulk_store_wait() {
   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
+// The same, and what was written is visible.
+__device__ __forceinline__ void bulk_store_done() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
 // A cluster barrier in two halves; the arrival orders no memory access.
 __device__ __forceinline__ void cluster_arrive_relaxed() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
