@@ -502,8 +502,8 @@ rtc_result rtc_embedding(const rtc_tensor* weight, const rtc_tensor* ids, float 
  * grad_output[i, :] over the i with ids[i] == v, in f32, in an order that
  * depends on ids alone), 0 for a v that no id names; with accumulate != 0 that
  * is added to grad_weight, and rows that no id names are not touched.  Ids
- * equal to padding_idx (negative: none) contribute nothing.  grad_output (ids' shape, D)
- * in T; grad_weight [V, D] in f32 or in T; fewer than 2^31 ids. */
+ * equal to padding_idx (negative: none) contribute nothing.  grad_output (ids'
+ * shape, D) in T; grad_weight [V, D] in f32 or in T; fewer than 2^31 ids. */
 rtc_result rtc_embedding_backward(const rtc_tensor* grad_output, const rtc_tensor* ids,
                                   float scale, int64_t padding_idx, int accumulate,
                                   const rtc_tensor* grad_weight);
@@ -552,7 +552,7 @@ rtc_result rtc_softmax_cross_entropy_grad(const rtc_tensor* logits, const rtc_te
  *    are a function of (seed, i, element) alone.  A non-zero r never becomes 0;
  *    a moment that is not finite is stored as NaN and leaves its block's scale
  *    to the others.  rtc_adamw8_pack and _unpack convert from and to f32.
- * All tensors are checked before anything is launched. */
+ * At most 2^20 tensors; all are checked before anything is launched. */
 rtc_result rtc_adamw_update_multi(const rtc_tensor* params, const rtc_tensor* grads,
                                   const rtc_tensor* m, const rtc_tensor* v,
                                   const rtc_tensor* m_scales, const rtc_tensor* v_scales,

@@ -5,8 +5,8 @@ the same function names, argument meaning and error behaviour (every failure
 raises ValueError, here the RusttorchError subclass carrying the TensorError
 variant).  The difference is where the data lives: a `Tensor` here is a
 buffer in GPU memory (float32, unless a token operator says otherwise), and
-every op is one call into librusttorch_cuda.so (see include/rusttorch_cuda.h).  Ops are asynchronous on
-the calling thread's stream; `to_numpy()` and the scalar reductions wait.
+every op is one call into librusttorch_cuda.so (see include/rusttorch_cuda.h).
+Ops are asynchronous on the calling thread's stream; `to_numpy()` and the scalar reductions wait.
 """
 from __future__ import annotations
 
@@ -528,14 +528,15 @@ def cross_entropy_loss(predictions: Tensor, targets: Tensor, epsilon: float = 1e
 
 # ---- token operators ---------------------------------------------------------
 # Asynchronous; with `out`, `loss`, `stats` and `grad` given (buffers that a
-# training loop keeps) a call allocates nothing from Python.
+# training loop keeps) a call allocates nothing from Python.  The descriptors go
+# in as they are (_desc.ref): the arguments live until the call returns.
 def embedding(weight: Tensor, ids: Tensor, scale: float = 1.0, out: Tensor | None = None) -> Tensor:
     """weight[ids] * scale: weight [V, D] in float32, bfloat16 or float16, ids
     of any shape in int32 or int64."""
     if out is None:
         width = weight.shape()[1:] if weight.ndim() == 2 else []
         out = Tensor(ids.shape() + width, weight.device, dtype=weight.dtype)
-    check(lib().rtc_embedding(weight.desc, ids.desc, float(scale), out.desc))
+    check(lib().rtc_embedding(weight._desc.ref, ids._desc.ref, float(scale), out._desc.ref))
     return out
 
 
@@ -556,8 +557,8 @@ def embedding_backward(grad_output: Tensor, ids: Tensor, num_embeddings: int, sc
     padding = -1 if padding_idx is None else int(padding_idx)
     if padding_idx is not None and padding < 0:
         raise RusttorchError("padding_idx must not be negative", _native.INVALID_ARGUMENT)
-    check(lib().rtc_embedding_backward(grad_output.desc, ids.desc, float(scale), padding,
-                                       int(accumulate), out.desc))
+    check(lib().rtc_embedding_backward(grad_output._desc.ref, ids._desc.ref, float(scale), padding,
+                                       int(accumulate), out._desc.ref))
     return out
 
 
@@ -583,8 +584,8 @@ def softmax_cross_entropy(logits: Tensor, targets: Tensor, ignore_index: int = -
     loss = _loss_out(targets, reduction, loss)
     if stats is None:
         stats = Tensor(targets.shape() + [3], targets.device)
-    check(lib().rtc_softmax_cross_entropy(logits.desc, targets.desc, int(ignore_index), code,
-                                          loss.desc, stats.desc))
+    check(lib().rtc_softmax_cross_entropy(logits._desc.ref, targets._desc.ref, int(ignore_index),
+                                          code, loss._desc.ref, stats._desc.ref))
     return loss, stats
 
 
@@ -595,8 +596,9 @@ def softmax_cross_entropy_backward(grad_output: Tensor, logits: Tensor, targets:
     code = _reduction(reduction)
     if out is None:
         out = Tensor(logits.shape(), logits.device, dtype=logits.dtype)
-    check(lib().rtc_softmax_cross_entropy_backward(grad_output.desc, logits.desc, targets.desc,
-                                                   stats.desc, int(ignore_index), code, out.desc))
+    check(lib().rtc_softmax_cross_entropy_backward(
+        grad_output._desc.ref, logits._desc.ref, targets._desc.ref, stats._desc.ref,
+        int(ignore_index), code, out._desc.ref))
     return out
 
 
@@ -610,8 +612,9 @@ def softmax_cross_entropy_grad(logits: Tensor, targets: Tensor, ignore_index: in
     loss = _loss_out(targets, reduction, loss)
     if grad is None:
         grad = Tensor(logits.shape(), logits.device, dtype=logits.dtype)
-    check(lib().rtc_softmax_cross_entropy_grad(logits.desc, targets.desc, int(ignore_index), code,
-                                               float(grad_scale), loss.desc, grad.desc))
+    check(lib().rtc_softmax_cross_entropy_grad(logits._desc.ref, targets._desc.ref,
+                                               int(ignore_index), code, float(grad_scale),
+                                               loss._desc.ref, grad._desc.ref))
     return loss, grad
 
 
@@ -637,7 +640,8 @@ def adamw8_pack(m: Tensor, v: Tensor) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     blocks = [-(-m.numel() // _native.MOMENT_BLOCK)]
     mc, vc = (Tensor(m.shape(), m.device, dtype="float8_e4m3") for _ in range(2))
     ms, vs = Tensor(blocks, m.device), Tensor(blocks, m.device)
-    check(lib().rtc_adamw8_pack(m.desc, v.desc, mc.desc, ms.desc, vc.desc, vs.desc))
+    check(lib().rtc_adamw8_pack(m._desc.ref, v._desc.ref, mc._desc.ref, ms._desc.ref, vc._desc.ref,
+                                vs._desc.ref))
     return mc, ms, vc, vs
 
 
@@ -645,8 +649,8 @@ def adamw8_unpack(m_codes: Tensor, m_scales: Tensor, v_codes: Tensor,
                   v_scales: Tensor) -> tuple[Tensor, Tensor]:
     """The float32 moments that adamw8_pack's or a step's codes stand for."""
     m, v = _like(m_codes), _like(m_codes)
-    check(lib().rtc_adamw8_unpack(m_codes.desc, m_scales.desc, v_codes.desc, v_scales.desc, m.desc,
-                                  v.desc))
+    check(lib().rtc_adamw8_unpack(m_codes._desc.ref, m_scales._desc.ref, v_codes._desc.ref,
+                                  v_scales._desc.ref, m._desc.ref, v._desc.ref))
     return m, v
 
 

@@ -1,5 +1,5 @@
 // rt_types.cuh — the storage types of the token operators: conversions to and
-// from f32, and 16-byte groups of elements.
+// from f32; and token ids.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -24,24 +24,6 @@ template <>
 __device__ __forceinline__ bf16 from_f32<bf16>(float x) { return __float2bfloat16_rn(x); }
 template <>
 __device__ __forceinline__ f16 from_f32<f16>(float x) { return __float2half_rn(x); }
-
-// 16 bytes of elements, moved by one load or store.
-template <class T>
-struct alignas(16) Pack {
-  static constexpr int N = 16 / sizeof(T);
-  T x[N];
-};
-
-// Loads and stores that each touch their bytes once (evict-first).
-template <class T>
-__device__ __forceinline__ Pack<T> ld_pack(const T* p) {
-  const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
-  return *reinterpret_cast<const Pack<T>*>(&v);
-}
-template <class T>
-__device__ __forceinline__ void st_pack(T* p, const Pack<T>& v) {
-  __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&v));
-}
 
 // Ids and targets: 32- or 64-bit integers, read as 64.
 struct IndexArray {

@@ -362,6 +362,12 @@ row_kernel(const T* logits, LossArgs a, unsigned each) {
   long long ahead = target_at(row + clusters);
   bool fine = true, counted = false;
   float scale = a.grad_scale;
+  if (a.count_here && (GRAD || blockIdx.x == 0)) {
+    const Count c = count_rows<TH>(a.targets, a.rows, a.ignore);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.count = c;
+    scale = fmul(scale, c.inverse);
+    counted = true;
+  }
   auto scale_by_count = [&] {
     if (!counted && a.count) {
       wait_for_previous_kernel();
@@ -396,9 +402,12 @@ row_kernel(const T* logits, LossArgs a, unsigned each) {
     const float xt = now.xt;
 
     Top<T> seen;
-#pragma unroll 4
+#pragma unroll 2
     for (unsigned i = threadIdx.x; i < count; i += TH) seen.see(run[i]);
-    const float m = warp_max(fmaxf(seen.get(), now.xe));
+    // The target's logit goes in with every warp, so that it has been read by
+    // all of them before a block of the cluster, which needs this warp's pair,
+    // may write its gradient in its place.
+    const float m = warp_max(fmaxf(fmaxf(seen.get(), now.xe), tg.t >= 0 ? xt : -INFINITY));
     // the target's place: a vector of this thread's, or its odd element
     float xe = now.xe;
     bool owner = false;
@@ -416,7 +425,7 @@ row_kernel(const T* logits, LossArgs a, unsigned each) {
     const Under um = under(against(m));
     F2 s2 = f2_of(0.0f, 0.0f);
     if (!um.wide) {
-#pragma unroll 4
+#pragma unroll 2
       for (unsigned i = threadIdx.x; i < count; i += TH) add_terms<false>(run[i], um, s2);
     } else {
 #pragma unroll 1
@@ -463,7 +472,7 @@ row_kernel(const T* logits, LossArgs a, unsigned each) {
       const float kf = fmul(k, ut.factor);
       const F2 k2 = f2_of(kf, kf);
       if (a.alike && !ut.wide && tg.counted) {
-#pragma unroll 4
+#pragma unroll 2
         for (unsigned i = threadIdx.x; i < count; i += TH)
           store_vec(gv + (size_t)i * N, scaled_terms<false>(run[i], ut, k2));
       } else {
@@ -566,7 +575,7 @@ template <class T>
 __global__ void __launch_bounds__(kThreads)
 token_grad_kernel(const T* logits, IndexArray targets, size_t rows, unsigned vocab,
                   long long ignore, const float* stats, const float* upstream, bool per_row,
-                  float grad_scale, const Count* count, T* grad, bool alike,
+                  float grad_scale, const Count* count, bool count_here, T* grad, bool alike,
                   unsigned parts, bool chained, int* bad) {
   constexpr int N = Vec<T>::N;
   constexpr int U = 4;
@@ -586,7 +595,8 @@ token_grad_kernel(const T* logits, IndexArray targets, size_t rows, unsigned voc
   if (chained) wait_for_previous_kernel();
   const float top = stats[3 * row], sum = stats[3 * row + 1], others = stats[3 * row + 2];
   float k = upstream ? upstream[per_row ? row : 0] : grad_scale;
-  if (count) k = fmul(k, count->inverse);
+  if (count_here) k = fmul(k, count_rows<kThreads>(targets, rows, ignore).inverse);
+  else if (count) k = fmul(k, count->inverse);
   k = tg.bad ? nan_f() : fmul(k, reciprocal(sum));
   if (tg.bad && part == 0 && threadIdx.x == 0) atomicExch(bad, 1);
   const Under ut = under(top);
@@ -669,12 +679,23 @@ cudaError_t rows_of(const TokenLoss& t, const LossArgs& a, bool chained, cudaStr
 // two blocks to an SM, and of one where eight of those are too few.
 template <class T, bool GRAD>
 cudaError_t rows_by_size(const TokenLoss& t, const LossArgs& a, bool chained, cudaStream_t s) {
-  const size_t vecs = vecs_of(t);
-  if (vecs <= run_vecs(16)) return rows_of<T, GRAD, 32, 16>(t, a, chained, s);
-  if (vecs <= run_vecs(8)) return rows_of<T, GRAD, 64, 8>(t, a, chained, s);
-  if (vecs <= run_vecs(4)) return rows_of<T, GRAD, 128, 4>(t, a, chained, s);
-  if (vecs <= kMaxCluster * run_vecs(2)) return rows_of<T, GRAD, 256, 2>(t, a, chained, s);
-  return rows_of<T, GRAD, 512, 1>(t, a, chained, s);
+  switch (row_threads(t)) {
+    case 32: return rows_of<T, GRAD, 32, 16>(t, a, chained, s);
+    case 64: return rows_of<T, GRAD, 64, 8>(t, a, chained, s);
+    case 128: return rows_of<T, GRAD, 128, 4>(t, a, chained, s);
+    case 256: {
+      // Three blocks to an SM where that puts more rows on it than two do, for
+      // 16-bit types (8192 x 32768 bf16: 207 us for 239; at 50257 both put one
+      // there, and three take 322 us for 312).  f32, whose time is HBM's, stays
+      // with two (4096 x 32768: 168 us for 177).
+      const size_t two = (vecs_of(t) + run_vecs(2) - 1) / run_vecs(2);
+      const size_t three = (vecs_of(t) + run_vecs(3) - 1) / run_vecs(3);
+      if (sizeof(T) == 2 && three <= kMaxCluster && 3 * two > 2 * three)
+        return rows_of<T, GRAD, 256, 3>(t, a, chained, s);
+      return rows_of<T, GRAD, 256, 2>(t, a, chained, s);
+    }
+    default: return rows_of<T, GRAD, 512, 1>(t, a, chained, s);
+  }
 }
 
 template <class T>
@@ -694,8 +715,8 @@ cudaError_t rows_any(const TokenLoss& t, const LossArgs& a, bool chained, cudaSt
 
 template <class T>
 cudaError_t grad_of(const TokenLoss& a, const float* stats, const float* upstream,
-                    float grad_scale, const Count* count, void* grad, bool chained,
-                    cudaStream_t s) {
+                    float grad_scale, const Count* count, bool count_here, void* grad,
+                    bool chained, cudaStream_t s) {
   const size_t parts = std::max<size_t>(1, (vecs_of(a) + 4 * kThreads - 1) / (4 * kThreads));
   const size_t step = std::max<size_t>(1, kMaxGrid / parts);
   const bool alike =
@@ -713,12 +734,12 @@ cudaError_t grad_of(const TokenLoss& a, const float* stats, const float* upstrea
     cudaError_t e;
     if (chained && r0 == 0) {
       e = launch_after(token_grad_kernel<T>, grid, kThreads, 0, s, x, targets, rows,
-                       (unsigned)a.vocab, a.ignore, stats, up, per_row, grad_scale, count, g,
-                       alike, (unsigned)parts, true, a.bad);
+                       (unsigned)a.vocab, a.ignore, stats, up, per_row, grad_scale, count,
+                       count_here, g, alike, (unsigned)parts, true, a.bad);
     } else {
       token_grad_kernel<T><<<grid, kThreads, 0, s>>>(
           x, targets, rows, (unsigned)a.vocab, a.ignore, stats + 3 * r0, up, per_row, grad_scale,
-          count, g, alike, (unsigned)parts, false, a.bad);
+          count, count_here, g, alike, (unsigned)parts, false, a.bad);
       e = cudaGetLastError();
     }
     if (e != cudaSuccess) return e;
@@ -735,9 +756,9 @@ cudaError_t grad_of(const TokenLoss& a, const float* stats, const float* upstrea
     return rows_any<T>(t, a, chained, s);                                                       \
   }                                                                                             \
   cudaError_t token_grad_##NAME(const TokenLoss& t, const float* stats, const float* upstream,  \
-                                float grad_scale, const Count* count, void* grad, bool chained, \
-                                cudaStream_t s) {                                               \
-    return grad_of<T>(t, stats, upstream, grad_scale, count, grad, chained, s);                 \
+                                float grad_scale, const Count* count, bool count_here,          \
+                                void* grad, bool chained, cudaStream_t s) {                     \
+    return grad_of<T>(t, stats, upstream, grad_scale, count, count_here, grad, chained, s);     \
   }
 
 }  // namespace rt

@@ -21,7 +21,8 @@ struct LossArgs {
   float* stats;                        // null, or [rows, 3]
   void* grad;                          // null, or the gradient
   float grad_scale;
-  const Count* count;                  // null, or what a mean divides by
+  Count* count;                        // null, or what a mean divides by
+  bool count_here;                     // the row kernel counts, and writes it
   int* bad;
   int* gave_up;                        // the flag of a wait that ran out
   bool alike;                          // grad's rows start where logits' do, modulo 16 bytes
@@ -33,8 +34,8 @@ struct LossArgs {
   cudaError_t token_rows_##NAME(const TokenLoss& t, const LossArgs& a, bool chained,            \
                                 cudaStream_t s);                                                \
   cudaError_t token_grad_##NAME(const TokenLoss& t, const float* stats, const float* upstream,  \
-                                float grad_scale, const Count* count, void* grad, bool chained, \
-                                cudaStream_t s);
+                                float grad_scale, const Count* count, bool count_here,          \
+                                void* grad, bool chained, cudaStream_t s);
 RT_TOKEN_LOSS_DECL(f32)
 RT_TOKEN_LOSS_DECL(bf16)
 RT_TOKEN_LOSS_DECL(f16)
@@ -53,6 +54,34 @@ inline size_t vecs_of(const TokenLoss& a) { return (a.vocab * store_bytes(a.type
 // Whether a row fits on chip, so that one pass gives its gradient too.
 inline bool fits_cluster(const TokenLoss& a) {
   return vecs_of(a) <= kMaxCluster * run_vecs(1);
+}
+
+// Threads of the blocks that take such rows (rows_by_size).
+inline int row_threads(const TokenLoss& a) {
+  const size_t vecs = vecs_of(a);
+  return vecs <= run_vecs(16)                 ? 32
+         : vecs <= run_vecs(8)                ? 64
+         : vecs <= run_vecs(4)                ? 128
+         : vecs <= kMaxCluster * run_vecs(2) ? 256 : 512;
+}
+
+// How many of `rows` targets are not `ignore`, at least 1, in all threads of a
+// block of TH; every thread calls it.
+template <int TH>
+__device__ __forceinline__ Count count_rows(const IndexArray& targets, size_t rows,
+                                            long long ignore) {
+  __shared__ unsigned part[TH / 32];
+  unsigned c = 0;
+#pragma unroll 8
+  for (size_t i = threadIdx.x; i < rows; i += TH) c += targets[i] != ignore;
+  c = __reduce_add_sync(0xffffffffu, c);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = c;
+  __syncthreads();
+  unsigned long long n = 0;
+#pragma unroll
+  for (int k = 0; k < TH / 32; k++) n += part[k];
+  n = n ? n : 1;
+  return {n, __frcp_rn((float)n)};
 }
 
 }  // namespace rt
