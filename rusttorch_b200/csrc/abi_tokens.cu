@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <new>
 
 using namespace rt;
 
@@ -20,28 +21,48 @@ bool store_type(int dtype, StoreType* t) {
   return false;
 }
 
-rtc_result need_float(const rtc_tensor* t, const std::string& what, StoreType* out) {
+// What an error is about: "op (argument)", or a name by itself.  Put together
+// for an error alone.
+struct What {
+  const char* op;
+  const char* argument;
+  std::string text;
+  What(const char* o, const char* a) : op(o), argument(a) {}
+  What(std::string t) : op(nullptr), argument(nullptr), text(std::move(t)) {}
+  std::string get() const {
+    return op ? std::string(op) + " (" + argument + ")" : text;
+  }
+};
+
+rtc_result need_float(const rtc_tensor* t, const What& what, StoreType* out) {
   if (!store_type(t->dtype, out))
-    return dtype_mismatch(what, "float32, bfloat16 or float16", dtype_display(t->dtype));
+    return dtype_mismatch(what.get(), "float32, bfloat16 or float16", dtype_display(t->dtype));
   return ok();
 }
 
-rtc_result need_ids(const rtc_tensor* t, const std::string& what) {
+rtc_result need_ids(const rtc_tensor* t, const What& what) {
   if (t->dtype != RTC_I32 && t->dtype != RTC_I64)
-    return dtype_mismatch(what, "int32 or int64", dtype_display(t->dtype));
+    return dtype_mismatch(what.get(), "int32 or int64", dtype_display(t->dtype));
   return ok();
 }
 
-rtc_result need_dtype(const rtc_tensor* t, int dtype, const std::string& what) {
+rtc_result need_dtype(const rtc_tensor* t, int dtype, const What& what) {
   if (t->dtype != dtype)
-    return dtype_mismatch(what, dtype_display(dtype), dtype_display(t->dtype));
+    return dtype_mismatch(what.get(), dtype_display(dtype), dtype_display(t->dtype));
   return ok();
 }
 
-rtc_result need_shape(const rtc_tensor* t, const std::vector<size_t>& shape,
-                      const std::string& what) {
-  if (shape_vec(t) != shape) return shape_mismatch_vec(what, shape, shape_vec(t));
-  return ok();
+// t has `lead`'s shape, then `last` unless that is kNone.
+constexpr size_t kNone = ~size_t(0);
+rtc_result need_shape(const rtc_tensor* t, const rtc_tensor* lead, size_t last,
+                      const What& what) {
+  const size_t extra = last != kNone;
+  bool same = t->ndim == lead->ndim + extra && (!extra || t->shape[lead->ndim] == last);
+  for (size_t i = 0; same && i < lead->ndim; i++) same = t->shape[i] == lead->shape[i];
+  if (same) return ok();
+  std::vector<size_t> want = shape_vec(lead);
+  if (extra) want.push_back(last);
+  return shape_mismatch_vec(what.get(), want, shape_vec(t));
 }
 
 rtc_result one_device(const rtc_tensor* a, const rtc_tensor* b) {
@@ -60,19 +81,23 @@ rtc_result apart_or_same(const rtc_tensor* out, const rtc_tensor* in, const char
   return out->data == in->data ? ok() : apart(out, in, what);
 }
 
-std::vector<size_t> with_last(const rtc_tensor* t, size_t last) {
-  std::vector<size_t> s = shape_vec(t);
-  s.push_back(last);
-  return s;
-}
-
 constexpr size_t kMaxVocab = 0x7fffffff;
+
+// What a first call sets up (the memory pool, attributes of kernels, occupancy)
+// queues nothing: a capture in progress, this thread's or another's, need not
+// end for it.
+struct SetupInCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  SetupInCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~SetupInCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
 
 // Runs launch(scratch, flag) on the tensors' device.
 template <class F>
 rtc_result on_device(int device, size_t scratch_bytes, const char* what, F launch) {
   DeviceScope scope(device);
   if (!scope.ok()) return backend_error("cudaSetDevice", scope.error());
+  SetupInCapture setup;
   int* bad = bad_index_flag(device);
   if (!bad) return backend_error(what, cudaErrorInvalidValue);
   if (scratch_bytes == 0) return launched(launch(nullptr, bad), what);
@@ -93,14 +118,14 @@ extern "C" rtc_result rtc_embedding(const rtc_tensor* weight, const rtc_tensor* 
   TRY(check_token_desc(ids, "ids"));
   TRY(check_token_desc(out, "out"));
   StoreType type;
-  TRY(need_float(weight, "embedding (weight)", &type));
-  TRY(need_ids(ids, "embedding (ids)"));
-  TRY(need_dtype(out, weight->dtype, "embedding (output)"));
+  TRY(need_float(weight, {"embedding", "weight"}, &type));
+  TRY(need_ids(ids, {"embedding", "ids"}));
+  TRY(need_dtype(out, weight->dtype, {"embedding", "output"}));
   if (weight->ndim != 2)
     return invalid_argument("weight", "must have two dimensions, got " +
                                           std::to_string(weight->ndim));
   const size_t vocab = weight->shape[0], width = weight->shape[1];
-  TRY(need_shape(out, with_last(ids, width), "embedding (output)"));
+  TRY(need_shape(out, ids, width, {"embedding", "output"}));
   if (vocab > kMaxVocab) return invalid_argument("weight", "must have fewer than 2^31 rows");
   TRY(one_device(weight, ids));
   TRY(one_device(weight, out));
@@ -122,9 +147,9 @@ extern "C" rtc_result rtc_embedding_backward(const rtc_tensor* grad_output, cons
   TRY(check_token_desc(ids, "ids"));
   TRY(check_token_desc(grad_weight, "grad_weight"));
   StoreType type, wtype;
-  TRY(need_float(grad_output, "embedding_backward (grad_output)", &type));
-  TRY(need_ids(ids, "embedding_backward (ids)"));
-  TRY(need_float(grad_weight, "embedding_backward (grad_weight)", &wtype));
+  TRY(need_float(grad_output, {"embedding_backward", "grad_output"}, &type));
+  TRY(need_ids(ids, {"embedding_backward", "ids"}));
+  TRY(need_float(grad_weight, {"embedding_backward", "grad_weight"}, &wtype));
   if (wtype != kF32 && wtype != type)
     return dtype_mismatch("embedding_backward (grad_weight)",
                           "float32 or " + dtype_display(grad_output->dtype),
@@ -133,7 +158,7 @@ extern "C" rtc_result rtc_embedding_backward(const rtc_tensor* grad_output, cons
     return invalid_argument("grad_weight", "must have two dimensions, got " +
                                                std::to_string(grad_weight->ndim));
   const size_t vocab = grad_weight->shape[0], width = grad_weight->shape[1];
-  TRY(need_shape(grad_output, with_last(ids, width), "embedding_backward (grad_output)"));
+  TRY(need_shape(grad_output, ids, width, {"embedding_backward", "grad_output"}));
   if (vocab > kMaxVocab) return invalid_argument("grad_weight", "must have fewer than 2^31 rows");
   if (ids->numel > kMaxVocab) return invalid_argument("ids", "must be fewer than 2^31");
   if (padding_idx >= 0 && (size_t)padding_idx >= vocab)
@@ -159,16 +184,16 @@ extern "C" rtc_result rtc_embedding_backward(const rtc_tensor* grad_output, cons
 namespace {
 
 rtc_result check_loss(const rtc_tensor* logits, const rtc_tensor* targets, int64_t ignore_index,
-                      int reduction, const std::string& ctx, TokenLoss* a) {
+                      int reduction, const char* ctx, TokenLoss* a) {
   TRY(check_token_desc(logits, "logits"));
   TRY(check_token_desc(targets, "targets"));
-  TRY(need_float(logits, ctx + " (logits)", &a->type));
-  TRY(need_ids(targets, ctx + " (targets)"));
+  TRY(need_float(logits, {ctx, "logits"}, &a->type));
+  TRY(need_ids(targets, {ctx, "targets"}));
   if (reduction < RTC_REDUCE_NONE || reduction > RTC_REDUCE_SUM)
     return invalid_argument("reduction", "must be RTC_REDUCE_NONE, _MEAN or _SUM");
   if (logits->ndim == 0) return invalid_argument("logits", "must have a last dimension");
   const size_t vocab = logits->shape[logits->ndim - 1];
-  TRY(need_shape(logits, with_last(targets, vocab), ctx + " (logits vs targets)"));
+  TRY(need_shape(logits, targets, vocab, {ctx, "logits vs targets"}));
   if (vocab == 0) return empty_tensor(ctx);
   if (vocab > kMaxVocab) return invalid_argument("logits", "must have fewer than 2^31 classes");
   TRY(one_device(logits, targets));
@@ -186,31 +211,31 @@ rtc_result check_loss(const rtc_tensor* logits, const rtc_tensor* targets, int64
 // One f32 per row, or one in all.
 rtc_result check_row_values(const rtc_tensor* t, const rtc_tensor* logits,
                             const rtc_tensor* targets, int reduction, const char* name,
-                            const std::string& ctx) {
+                            const char* ctx) {
   TRY(check_token_desc(t, name));
-  TRY(need_dtype(t, RTC_F32, ctx + " (" + name + ")"));
+  TRY(need_dtype(t, RTC_F32, {ctx, name}));
   if (reduction == RTC_REDUCE_NONE)
-    TRY(need_shape(t, shape_vec(targets), ctx + " (" + name + ")"));
+    TRY(need_shape(t, targets, kNone, {ctx, name}));
   else if (t->numel != 1)
     return invalid_argument(name, "must have one element, got " + std::to_string(t->numel));
   return one_device(logits, t);
 }
 
 rtc_result check_grad_logits(const rtc_tensor* logits, const rtc_tensor* targets,
-                             const rtc_tensor* grad, const std::string& ctx) {
+                             const rtc_tensor* grad, const char* ctx) {
   TRY(check_token_desc(grad, "grad_logits"));
-  TRY(need_dtype(grad, logits->dtype, ctx + " (grad_logits)"));
-  TRY(need_shape(grad, shape_vec(logits), ctx + " (grad_logits)"));
+  TRY(need_dtype(grad, logits->dtype, {ctx, "grad_logits"}));
+  TRY(need_shape(grad, logits, kNone, {ctx, "grad_logits"}));
   TRY(one_device(logits, grad));
   TRY(apart(grad, targets, "grad_logits"));
   return apart_or_same(grad, logits, "grad_logits");
 }
 
 rtc_result check_stats(const rtc_tensor* stats, const rtc_tensor* logits,
-                       const rtc_tensor* targets, const std::string& ctx) {
+                       const rtc_tensor* targets, const char* ctx) {
   TRY(check_token_desc(stats, "stats"));
-  TRY(need_dtype(stats, RTC_F32, ctx + " (stats)"));
-  TRY(need_shape(stats, with_last(targets, 3), ctx + " (stats)"));
+  TRY(need_dtype(stats, RTC_F32, {ctx, "stats"}));
+  TRY(need_shape(stats, targets, 3, {ctx, "stats"}));
   return one_device(logits, stats);
 }
 
@@ -338,10 +363,6 @@ rtc_result check_moments(const rtc_tensor* p, const rtc_tensor* codes, const rtc
   return one_device(p, scales);
 }
 
-}  // namespace
-
-namespace {
-
 // Tensor i of the lists, with the errors that its checks give.
 rtc_result check_listed(const rtc_tensor* params, const rtc_tensor* grads, const rtc_tensor* m,
                         const rtc_tensor* v, const rtc_tensor* m_scales,
@@ -416,7 +437,7 @@ extern "C" rtc_result rtc_adamw_update_multi(
     const rtc_tensor* params, const rtc_tensor* grads, const rtc_tensor* m, const rtc_tensor* v,
     const rtc_tensor* m_scales, const rtc_tensor* v_scales, const rtc_tensor* copies, size_t n,
     double learning_rate, double beta1, double beta2, double epsilon, double weight_decay,
-    uint64_t timestep, uint64_t seed) {
+    uint64_t timestep, uint64_t seed) try {
   RTC_OP_RANGE();
   if (n == 0) return ok();
   if (!params) return invalid_argument("params", "must not be null");
@@ -485,6 +506,8 @@ extern "C" rtc_result rtc_adamw_update_multi(
     return launch_adam8_multi(list.data(), n, c8, seed, wait_timeout_flag(params[0].device),
                               thread_stream());
   });
+} catch (const std::bad_alloc&) {   // the lists' copies
+  return backend_error("adamw_update_multi", cudaErrorMemoryAllocation);
 }
 
 namespace {
@@ -494,8 +517,8 @@ rtc_result check_packed(const rtc_tensor* m, const rtc_tensor* v, const rtc_tens
   TRY(check_token_desc(v, "v"));
   TRY(check_token_desc(mc, "m_codes"));
   TRY(check_token_desc(vc, "v_codes"));
-  TRY(need_dtype(m, RTC_F32, "m"));
-  TRY(need_dtype(v, RTC_F32, "v"));
+  TRY(need_dtype(m, RTC_F32, What("m")));
+  TRY(need_dtype(v, RTC_F32, What("v")));
   if (!same_shape(m, v)) return shape_mismatch("v", m, v);
   if (!same_shape(m, mc)) return shape_mismatch("m_codes", m, mc);
   if (!same_shape(m, vc)) return shape_mismatch("v_codes", m, vc);

@@ -519,6 +519,7 @@ adam8_multi_kernel(const __grid_constant__ Table<CAP> tab, Adam8Coeffs c, unsign
     for (unsigned u = blockIdx.x; u < units && fine; u += gridDim.x, turn++) {
       Stage8& st = stages[turn % kStages];
       if (turn >= kStages) fine = mbar_wait(&st.empty, (turn / kStages - 1) & 1);
+      if (!fine) break;
       const int k = tensor_of(tab, u);
       const AdamTensor& t = tab.t[k];
       const size_t begin = (size_t)(u - tab.first[k]) * kUnit;

@@ -407,6 +407,22 @@ def test_embedding_gradient_of_misaligned_tensors(rt, a, b, dtype):
     assert (around[:b] == 9).all() and (around[b + want.size:] == 9).all()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("v, d", [(1, 1), (6, 1), (5, 3), (13, 1), (4, 31)])
+def test_embedding_gradient_of_small_tables_anywhere(rt, v, d, dtype):
+    """Every start modulo 16 bytes: all of the table is written, nothing around it."""
+    g = K.rounded(np.arange(1, d + 1, dtype=np.float32)[None], dtype)
+    G, I = put(rt, g, dtype), rt.Tensor.from_numpy(np.array([v // 2]))
+    want = np.zeros((v, d), np.float32)
+    want[v // 2] = g
+    for b in range(16 // N.DTYPE_BYTES[G._code]):
+        O, big = shifted(rt, np.full((v, d), 5.0), dtype, b)
+        rt.embedding_backward(G, I, v, out=O)
+        same(get(O), want)
+        around = get(big)
+        assert (around[:b] == 9).all() and (around[b + want.size:] == 9).all()
+
+
 def test_embedding_gradient_without_ids(rt):
     out = rt.Tensor.from_numpy(np.ones((5, 6), np.float32))
     rt.embedding_backward(rt.Tensor([0, 6]), rt.Tensor([0], dtype="int64"), 5, accumulate=True, out=out)
@@ -751,3 +767,62 @@ def test_two_calls_at_once(rt):
     for s, w in zip(states, plain):
         for x, y in zip(results(s), results(w)):
             assert (x == y).all()
+
+
+FIRST = """
+import ctypes, sys
+import torch
+import rusttorch_b200 as rt
+from rusttorch_b200 import _native as N
+f = lambda *shape, t=torch.float32: (torch.rand(shape, device="cuda") * 40).to(t)
+def wrap(x):
+    name = {torch.float32: "float32", torch.int64: "int64", torch.uint8: "float8_e4m3"}[x.dtype]
+    return rt.Tensor.from_device_ptr(x.data_ptr(), x.shape, owner=x, dtype=name)
+w, emb, loss, p, gr, m, v = f(50, 8), f(300, 8), f(1), f(400), f(400), f(400), f(400)
+x, g = f(300, 9000), f(300, 9000)
+ids, mc, vc, ms, vs = f(300, t=torch.int64), f(400, t=torch.uint8), f(400, t=torch.uint8), f(4), f(4)
+W, E, I, X, L, G, P, GR, M, V, MC, VC, MS, VS = map(wrap, (w, emb, ids, x, loss, g, p, gr, m, v, mc, vc, ms, vs))
+h = (1e-3, 0.9, 0.999, 1e-8, 0.01, 1)
+call = {
+    "embedding": lambda: rt.embedding(W, I, out=E),
+    "embedding_backward": lambda: rt.embedding_backward(E, I, 50, out=W),
+    "softmax_cross_entropy_grad": lambda: rt.softmax_cross_entropy_grad(X, I, loss=L, grad=G),
+    "adamw_update_multi": lambda: rt.adamw_update_multi([P], [GR], [M], [V], *h),
+    "adamw_update_multi_8": lambda: rt.adamw_update_multi([P], [GR], [MC], [VC], *h, m_scales=[MS], v_scales=[VS], seed=3),
+}[sys.argv[1]]
+outputs = (w, emb, loss, p, m, v, g, mc, vc, ms, vs)
+start = [y.clone() for y in outputs]
+stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph, stream=stream):
+    N.check(N.lib().rtc_set_stream(ctypes.c_void_p(stream.cuda_stream)))
+    call()
+    N.check(N.lib().rtc_set_stream(None))
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(outputs, start)), "it ran while it was captured"
+graph.replay()
+torch.cuda.synchronize()
+got = [y.clone() for y in outputs]
+assert not all(torch.equal(a, b) for a, b in zip(got, start))
+for y, a in zip(outputs, start):
+    y.copy_(a)
+torch.cuda.synchronize()
+call()
+N.check(N.lib().rtc_synchronize())
+assert all(torch.equal(a, b) for a, b in zip(outputs, got))
+del graph
+print("fine")
+"""
+
+
+@pytest.mark.parametrize("op", ["embedding", "embedding_backward", "softmax_cross_entropy_grad",
+                                "adamw_update_multi", "adamw_update_multi_8"])
+def test_first_call_of_a_process_is_captured(op):
+    """Nothing that a first call sets up may need a stream that is not capturing."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    pytest.importorskip("torch")
+    r = subprocess.run([sys.executable, "-c", FIRST, op], cwd=Path(__file__).resolve().parents[1],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("fine"), r.stderr[-2000:]
