@@ -170,7 +170,7 @@ extern "C" rtc_result rtc_embedding_backward(const rtc_tensor* grad_output, cons
   TRY(apart(grad_weight, grad_output, "grad_weight"));
   TRY(apart(grad_weight, ids, "grad_weight"));
   if (grad_weight->numel == 0) return ok();
-  return on_device(grad_output->device, embedding_backward_scratch(ids->numel, width), ctx,
+  return on_device(grad_output->device, embedding_backward_scratch(type, ids->numel, width), ctx,
                    [&](void* scratch, int* bad) {
                      return launch_embedding_backward(
                          type, grad_output->data, ids->data, ids->dtype == RTC_I64, ids->numel,
@@ -325,19 +325,44 @@ struct Range {
   const char* list;
 };
 
-void add_range(std::vector<Range>* r, const rtc_tensor* t, size_t i, const char* list) {
-  const uintptr_t b = reinterpret_cast<uintptr_t>(t->data);
-  if (t->numel) r->push_back({b, b + t->numel * dtype_bytes(t->dtype), i, list});
-}
+// Every tensor of a call, list by list.
+struct Ranges {
+  static constexpr int kLists = 7;
+  std::vector<Range> list[kLists];
+
+  explicit Ranges(size_t n) {
+    for (auto& l : list) l.reserve(n);
+  }
+  void add(int k, const rtc_tensor* t, size_t i, const char* name) {
+    const uintptr_t b = reinterpret_cast<uintptr_t>(t->data);
+    if (t->numel) list[k].push_back({b, b + t->numel * dtype_bytes(t->dtype), i, name});
+  }
+
+  // Whether each list's tensors follow one another in memory and no two lists'
+  // spans meet, as where a list was cut from one buffer.
+  bool laid_out() const {
+    for (const auto& l : list)
+      for (size_t i = 1; i < l.size(); i++)
+        if (l[i].begin < l[i - 1].end) return false;
+    for (int a = 0; a < kLists; a++)
+      for (int b = 0; b < a; b++)
+        if (!list[a].empty() && !list[b].empty() && list[a].front().begin < list[b].back().end &&
+            list[b].front().begin < list[a].back().end)
+          return false;
+    return true;
+  }
+};
 
 // No written tensor may share bytes with another (the same parameter twice in
 // one call, say): the blocks of both would race.
-rtc_result no_shared_writes(std::vector<Range>* r) {
-  std::sort(r->begin(), r->end(),
-            [](const Range& a, const Range& b) { return a.begin < b.begin; });
+rtc_result no_shared_writes(const Ranges& ranges) {
+  if (ranges.laid_out()) return ok();
+  std::vector<Range> r;
+  for (const auto& l : ranges.list) r.insert(r.end(), l.begin(), l.end());
+  std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
   const Range* written = nullptr;   // of those before: the written one, and the
   const Range* any = nullptr;       // one at all, that reach furthest
-  for (const Range& x : *r) {
+  for (const Range& x : r) {
     const Range* hit = written && written->end > x.begin ? written : nullptr;
     if (!hit && x.list && any && any->end > x.begin) hit = &x;
     if (hit)
@@ -410,11 +435,18 @@ bool plain(const rtc_tensor* t) {
     if (prod > SIZE_MAX) return false;
   }
   return prod == t->numel && (t->numel == 0 || t->data) &&
-         reinterpret_cast<uintptr_t>(t->data) % dtype_bytes(t->dtype) == 0;
+         (reinterpret_cast<uintptr_t>(t->data) & (dtype_bytes(t->dtype) - 1)) == 0;
 }
 bool plain_f32(const rtc_tensor* t) { return t->dtype == RTC_F32 && plain(t); }
+// p is plain.
 bool plain_like(const rtc_tensor* t, const rtc_tensor* p) {
-  return plain(t) && t->device == p->device && same_shape(t, p);
+  if (t->strides || t->device != p->device || t->ndim != p->ndim || t->numel != p->numel ||
+      (t->ndim > 0 && !t->shape))
+    return false;
+  for (size_t i = 0; i < t->ndim; i++)
+    if (t->shape[i] != p->shape[i]) return false;
+  return (t->numel == 0 || t->data) &&
+         (reinterpret_cast<uintptr_t>(t->data) & (dtype_bytes(t->dtype) - 1)) == 0;
 }
 bool plain_moment(const rtc_tensor* t, const rtc_tensor* p, bool eight) {
   return t->dtype == (eight ? RTC_F8E4M3 : RTC_F32) && plain_like(t, p);
@@ -452,8 +484,7 @@ extern "C" rtc_result rtc_adamw_update_multi(
   if (weight_decay < 0.0)
     return invalid_argument("weight_decay", "must be non-negative, got " + rust_f64(weight_decay));
   std::vector<AdamTensor> list(n);
-  std::vector<Range> ranges;
-  ranges.reserve(7 * n);
+  Ranges ranges(n);
   for (size_t i = 0; i < n; i++) {
     const rtc_tensor* p = &params[i];
     AdamTensor& t = list[i];
@@ -477,17 +508,17 @@ extern "C" rtc_result rtc_adamw_update_multi(
     t.m = m[i].data;
     t.v = v[i].data;
     t.n = p->numel;
-    add_range(&ranges, p, i, "params");
-    add_range(&ranges, &grads[i], i, nullptr);
-    add_range(&ranges, &m[i], i, "m");
-    add_range(&ranges, &v[i], i, "v");
+    ranges.add(0, p, i, "params");
+    ranges.add(1, &grads[i], i, nullptr);
+    ranges.add(2, &m[i], i, "m");
+    ranges.add(3, &v[i], i, "v");
     if (eight) {
-      add_range(&ranges, &m_scales[i], i, "m_scales");
-      add_range(&ranges, &v_scales[i], i, "v_scales");
+      ranges.add(4, &m_scales[i], i, "m_scales");
+      ranges.add(5, &v_scales[i], i, "v_scales");
     }
-    if (copies) add_range(&ranges, &copies[i], i, "copies");
+    if (copies) ranges.add(6, &copies[i], i, "copies");
   }
-  TRY(no_shared_writes(&ranges));
+  TRY(no_shared_writes(ranges));
   TRY(adam_hyper_checks(learning_rate, beta1, beta2, epsilon, timestep));
   return on_device(params[0].device, 0, "adamw_update_multi", [&](void*, int*) {
     const AdamCoeffs c =

@@ -21,7 +21,8 @@ namespace {
 
 constexpr int kChunk = 4096;       // elements to a block, moments in f32
 constexpr int kMaxTensors = 400;   // a launch; a kernel's arguments end at 32,764 bytes
-constexpr int kFewTensors = 32;    // short lists travel in a smaller argument
+constexpr int kFewTensors = 32;    // shorter lists travel in a smaller argument
+constexpr int kSomeTensors = 128;
 
 template <int CAP>
 struct Table {
@@ -667,8 +668,9 @@ cudaError_t launch_adam_multi(const AdamTensor* t, size_t n, const AdamCoeffs& c
     adam_multi_kernel<<<chunks, kThreads, 0, s>>>(tab, c);
     return cudaGetLastError();
   };
-  return n <= kFewTensors ? for_tables<kFewTensors>(t, n, kChunk, launch)
-                          : for_tables<kMaxTensors>(t, n, kChunk, launch);
+  return n <= kFewTensors    ? for_tables<kFewTensors>(t, n, kChunk, launch)
+         : n <= kSomeTensors ? for_tables<kSomeTensors>(t, n, kChunk, launch)
+                             : for_tables<kMaxTensors>(t, n, kChunk, launch);
 }
 
 namespace {
@@ -692,8 +694,9 @@ cudaError_t adam8_by_tables(const AdamTensor* t, size_t n, const Adam8Coeffs& c,
 
 cudaError_t launch_adam8_multi(const AdamTensor* t, size_t n, const Adam8Coeffs& c, uint64_t seed,
                                int* gave_up, cudaStream_t s) {
-  return n <= kFewTensors ? adam8_by_tables<kFewTensors>(t, n, c, seed, gave_up, s)
-                          : adam8_by_tables<kMaxTensors>(t, n, c, seed, gave_up, s);
+  return n <= kFewTensors    ? adam8_by_tables<kFewTensors>(t, n, c, seed, gave_up, s)
+         : n <= kSomeTensors ? adam8_by_tables<kSomeTensors>(t, n, c, seed, gave_up, s)
+                             : adam8_by_tables<kMaxTensors>(t, n, c, seed, gave_up, s);
 }
 
 cudaError_t launch_adam8_pack(const float* m, const float* v, void* mc, float* ms, void* vc,

@@ -1,12 +1,13 @@
 // embedding.cu — rows of a table by token id, and the table's gradient.
 //
 // Forward: out[i, :] = T(scale * weight[ids[i], :]), one f32 product and one
-// rounding per element.  A group of threads walks a row, 16 bytes a thread.
+// rounding per element, 16 bytes of a row a thread.  HBM bounds it (32768 x 4096
+// bf16 of 131072 rows: 68 us, 5.4 TB/s).
 //
 // Gradient: grad_weight[v, :] (+)= scale * sum over {i : ids[i] = v} of
 // grad_output[i, :].  The sums of a row are wherever its tokens are, so:
 //  1. sort_ids_kernel sorts the positions by id (stable radix sort) in one
-//     cluster of thread blocks;
+//     cluster of thread blocks, few_ids_kernel few of them by counting;
 //  2. segment_kernel cuts the sorted list into pieces of equal length, so
 //     that a frequent id costs no block more than a rare one; a group sums its
 //     piece's rows in order, writes each id's sum that begins and ends in the
@@ -47,7 +48,7 @@ struct Row {
   T x[N];
 };
 
-template <int VW, bool ONCE, class T>
+template <int VW, class T>
 __device__ __forceinline__ void load_row(const T* row, size_t first, unsigned G, size_t width,
                                          Row<T>& r) {
   constexpr int N = Row<T>::N;
@@ -58,8 +59,7 @@ __device__ __forceinline__ void load_row(const T* row, size_t first, unsigned G,
       const T* p = row + c;
       if constexpr (VW * sizeof(T) == 16) {
         const uint4* q = reinterpret_cast<const uint4*>(p);
-        const uint4 v = ONCE ? __ldcs(q) : __ldg(q);
-        *reinterpret_cast<uint4*>(&r.x[k * VW]) = v;
+        *reinterpret_cast<uint4*>(&r.x[k * VW]) = __ldcs(q);
       } else {
         const auto v = *reinterpret_cast<const Chunk<T, VW>*>(p);
 #pragma unroll
@@ -117,17 +117,15 @@ __device__ __forceinline__ void add_row(const G_* row, size_t first, unsigned G,
 
 // ---- forward -------------------------------------------------------------------
 
-// R rows to a group, one tile of G * 16 bytes of each.
-template <class T, int VW, int R>
+// Rows that all start on 16 bytes: a thread takes the same 16 bytes of R rows.
+template <class T, int R>
 __global__ void __launch_bounds__(kThreads)
 embedding_kernel(const T* w, IndexArray ids, size_t n, long long vocab, size_t width, float scale,
-                 T* out, int* bad, unsigned G, unsigned tiles) {
+                 T* out, int* bad, unsigned vecs) {
   constexpr int N = Row<T>::N;
-  const unsigned per_block = kThreads / G;
-  const size_t unit = (size_t)blockIdx.x * per_block + threadIdx.x / G;
-  const size_t i0 = unit / tiles * R;
-  const unsigned lane = threadIdx.x % G;
-  const size_t first = (size_t)(unit % tiles) * G * N + (size_t)lane * VW;
+  const size_t unit = (size_t)blockIdx.x * kThreads + threadIdx.x;
+  const size_t i0 = unit / vecs * R;
+  const size_t first = unit % vecs * N;
   Row<T> x[R];
   bool good[R];
 #pragma unroll
@@ -136,18 +134,103 @@ embedding_kernel(const T* w, IndexArray ids, size_t n, long long vocab, size_t w
     if (i0 + r < n) {
       const long long id = ids[i0 + r];
       good[r] = id >= 0 && id < vocab;
-      if (good[r]) load_row<VW, false>(w + (size_t)id * width, first, G, width, x[r]);
+      if (good[r])
+        *reinterpret_cast<uint4*>(x[r].x) =
+            __ldg(reinterpret_cast<const uint4*>(w + (size_t)id * width + first));
       else if (first == 0) atomicExch(bad, 1);
     }
   }
 #pragma unroll
   for (int r = 0; r < R; r++) {
     if (i0 + r < n) {
-      float v[N];
+      Row<T> o;
 #pragma unroll
       for (int e = 0; e < N; e++)
-        v[e] = good[r] ? fmul(to_f32(x[r].x[e]), scale) : u2f(0x7fc00000u);
-      store_row<VW>(out + (i0 + r) * width, first, G, width, v);
+        o.x[e] = from_f32<T>(good[r] ? fmul(to_f32(x[r].x[e]), scale) : u2f(0x7fc00000u));
+      *reinterpret_cast<uint4*>(out + (i0 + r) * width + first) =
+          *reinterpret_cast<const uint4*>(o.x);
+    }
+  }
+}
+
+// Rows that do not all start on 16 bytes: a thread takes 16 aligned bytes of the
+// output and reads them as two aligned 16-byte accesses, of which it shifts
+// together what it needs; elements beyond a row's ends are not stored.  Nothing
+// outside the table is read.  (32768 rows of 1023 bf16, 50257 in the table:
+// 31 us, and 53 us with an access for each element.)
+template <class T>
+__device__ __forceinline__ uint4 load_anywhere(const char* p) {
+  const unsigned off = reinterpret_cast<uintptr_t>(p) & 15;
+  const uint4* q = reinterpret_cast<const uint4*>(p - off);
+  uint4 a = __ldg(q);
+  if (off == 0) return a;
+  uint4 b = __ldg(q + 1);
+  if (off & 8) {
+    a = make_uint4(a.z, a.w, b.x, b.y);
+    b.x = b.z;
+    b.y = b.w;
+  }
+  if (off & 4) {
+    a = make_uint4(a.y, a.z, a.w, b.x);
+    b.x = b.y;
+  }
+  if (sizeof(T) == 2 && (off & 2))
+    a = make_uint4(__funnelshift_r(a.x, a.y, 16), __funnelshift_r(a.y, a.z, 16),
+                   __funnelshift_r(a.z, a.w, 16), __funnelshift_r(a.w, b.x, 16));
+  return a;
+}
+
+template <class T, int R>
+__global__ void __launch_bounds__(kThreads)
+embedding_anywhere_kernel(const T* w, IndexArray ids, size_t n, long long vocab, size_t width,
+                          float scale, T* out, int* bad, unsigned vecs) {
+  constexpr int N = Row<T>::N;
+  const size_t unit = (size_t)blockIdx.x * kThreads + threadIdx.x;
+  const size_t i0 = unit / vecs * R;
+  const unsigned vec = (unsigned)(unit % vecs);
+  const char* const begin = reinterpret_cast<const char*>(w);
+  const char* const end = reinterpret_cast<const char*>(w + (size_t)vocab * width);
+  Row<T> x[R];
+  long long e[R];        // the row's element that the 16 bytes begin with
+  bool good[R];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    good[r] = false;
+    e[r] = 0;
+    if (i0 + r >= n) continue;
+    const long long id = ids[i0 + r];
+    const uintptr_t to = reinterpret_cast<uintptr_t>(out + (i0 + r) * width);
+    e[r] = (long long)vec * N - (long long)((to & 15) / sizeof(T));
+    good[r] = id >= 0 && id < vocab;
+    if (good[r]) {
+      const long long at = id * (long long)width + e[r];   // in the table
+      const char* p = begin + at * (long long)sizeof(T);
+      const unsigned off = reinterpret_cast<uintptr_t>(p) & 15;
+      if (p - off >= begin && p + (off ? 32 - off : 16) <= end) {
+        *reinterpret_cast<uint4*>(x[r].x) = load_anywhere<T>(p);
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+          if (e[r] + k >= 0 && e[r] + k < (long long)width) x[r].x[k] = w[at + k];
+      }
+    } else if (vec == 0) {
+      atomicExch(bad, 1);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    if (i0 + r >= n) continue;
+    T* to = out + (i0 + r) * width + e[r];
+    Row<T> o;
+#pragma unroll
+    for (int k = 0; k < N; k++)
+      o.x[k] = from_f32<T>(good[r] ? fmul(to_f32(x[r].x[k]), scale) : u2f(0x7fc00000u));
+    if (e[r] >= 0 && e[r] + N <= (long long)width) {
+      *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(o.x);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; k++)
+        if (e[r] + k >= 0 && e[r] + k < (long long)width) to[k] = o.x[k];
     }
   }
 }
@@ -171,43 +254,30 @@ int chunk_of(size_t width, const void* a, size_t a_size, const void* b, size_t b
   return vw;
 }
 
-template <class T, int VW>
-cudaError_t embedding_of(const T* w, IndexArray ids, size_t n, size_t vocab, size_t width,
-                         float scale, T* out, int* bad, cudaStream_t s) {
-  constexpr int N = Row<T>::N;
-  const unsigned G = group_of(width, N);
-  const unsigned tiles = (unsigned)((width + (size_t)G * N - 1) / ((size_t)G * N));
-  const unsigned per_block = kThreads / G;
-  // Four rows a group keep 64 bytes a thread in flight; with few rows one each
-  // spreads them over more SMs.
-  int device = 0;
-  cudaGetDevice(&device);
-  const bool many = n * tiles >= (size_t)8 * sm_count(device) * per_block;
-  const size_t units = (many ? (n + 3) / 4 : n) * tiles;
-  const size_t blocks = (units + per_block - 1) / per_block;
-  if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
-  if (many)
-    embedding_kernel<T, VW, 4><<<(unsigned)blocks, kThreads, 0, s>>>(
-        w, ids, n, (long long)vocab, width, scale, out, bad, G, tiles);
-  else
-    embedding_kernel<T, VW, 1><<<(unsigned)blocks, kThreads, 0, s>>>(
-        w, ids, n, (long long)vocab, width, scale, out, bad, G, tiles);
-  return cudaGetLastError();
-}
-
 template <class T>
 cudaError_t embedding_any(const void* weight, IndexArray ids, size_t n, size_t vocab, size_t width,
                           float scale, void* out, int* bad, cudaStream_t s) {
+  constexpr int N = Row<T>::N;
   const T* w = static_cast<const T*>(weight);
   T* o = static_cast<T*>(out);
-  switch (chunk_of<T>(width, w, sizeof(T), o, sizeof(T))) {
-    case 8:
-      if constexpr (sizeof(T) == 2)
-        return embedding_of<T, 8>(w, ids, n, vocab, width, scale, o, bad, s);
-    case 4: return embedding_of<T, 4>(w, ids, n, vocab, width, scale, o, bad, s);
-    case 2: return embedding_of<T, 2>(w, ids, n, vocab, width, scale, o, bad, s);
-    default: return embedding_of<T, 1>(w, ids, n, vocab, width, scale, o, bad, s);
-  }
+  const bool aligned = chunk_of<T>(width, w, sizeof(T), o, sizeof(T)) == N;
+  // the 16 bytes that a row may touch: one more where it starts inside some
+  const size_t vecs = aligned ? width / N : (width + 2 * N - 2) / N;
+  // Four rows a thread keep 64 bytes of each in flight (two where each takes two
+  // accesses and more registers: 1001 f32 43 us, 58 with four, 52 with one); with
+  // few rows one each spreads them over more SMs.
+  int device = 0;
+  cudaGetDevice(&device);
+  const bool many = n * vecs >= (size_t)8 * sm_count(device) * kThreads;
+  const size_t rows = !many ? 1 : aligned ? 4 : 2;
+  const size_t blocks = ((n + rows - 1) / rows * vecs + kThreads - 1) / kThreads;
+  if (blocks > 0x7fffffffull || vecs > 0xffffffffull) return cudaErrorInvalidValue;
+  const auto kernel = aligned ? (many ? embedding_kernel<T, 4> : embedding_kernel<T, 1>)
+                              : (many ? embedding_anywhere_kernel<T, 2>
+                                      : embedding_anywhere_kernel<T, 1>);
+  kernel<<<(unsigned)blocks, kThreads, 0, s>>>(w, ids, n, (long long)vocab, width, scale, o, bad,
+                                               (unsigned)vecs);
+  return cudaGetLastError();
 }
 
 // ---- sorting ---------------------------------------------------------------------
@@ -422,11 +492,42 @@ sort_ids_kernel(IndexArray ids, unsigned n, long long vocab, long long padding, 
   }
 }
 
+// The same for at most 4096 without passes: a key's place is how many come
+// before it, which a warp counts for each key, 32 keys to a block.  The blocks
+// do not wait for one another.  (With the rest of the gradient of 1000
+// ids of 512 bf16: 17 us, and 27 us with the passes; of 4000: 24 and 31 us.)
+constexpr unsigned kFewIds = kShadowBytes / 4;
+__global__ void __launch_bounds__(kSortThreads)
+few_ids_kernel(IndexArray ids, unsigned n, long long vocab, long long padding, Sorted out,
+               unsigned sorting, Shadow shadow, int* bad) {
+  __shared__ uint4 buffer[kShadowBytes / 16];
+  let_next_kernel_start();
+  if (blockIdx.x >= sorting) {
+    write_shadow(shadow, buffer, blockIdx.x - sorting, gridDim.x - sorting);
+    return;
+  }
+  unsigned* key = reinterpret_cast<unsigned*>(buffer);
+  if (blockIdx.x == 0 && threadIdx.x < 2) out.count[threadIdx.x] = 0;
+#pragma unroll 4
+  for (unsigned j = threadIdx.x; j < n; j += kSortThreads)
+    key[j] = key_of(ids, j, vocab, padding, bad);
+  __syncthreads();
+  const unsigned i = blockIdx.x * kSortWarps + (threadIdx.x >> 5);
+  if (i >= n) return;
+  const unsigned k = key[i];
+  unsigned place = 0;
+#pragma unroll 4
+  for (unsigned j = threadIdx.x & 31; j < n; j += 32) place += key[j] < k + (j < i);
+  place = __reduce_add_sync(0xffffffffu, place);
+  if ((threadIdx.x & 31) == 0) out.pair[0][place] = make_uint2(k, i);
+}
+
 // ---- sums -------------------------------------------------------------------------
 
 constexpr int kSub = 16;             // sorted positions whose ids are staged at a time
-constexpr int kMinPiece = 32;
+constexpr int kPiece = 32;           // positions to a piece, unless there are few or very many
 constexpr size_t kMaxPieces = 2048;
+constexpr size_t kFewPieces = 1024;  // at most, where pieces are cut shorter than kPiece
 constexpr unsigned kLong = 16;       // a sum over more pieces than this is a long one
 constexpr int kZeroRows = 64;        // at most, to a block that writes zeros
 constexpr int kZeroBytes = 4096;     // zeros that it copies at a time
@@ -592,14 +693,16 @@ segment_kernel(const T* g, W* gw, Plan a) {
         if (k != none && (i == 0 || skey[i - 1] != k) && first < a.width)
           prefetch_l2(gw + (size_t)k * a.width + first);
       }
-    for (unsigned i = 0; i < kSub; i += U) {
+    const unsigned turn = min((unsigned)kSub, a.piece);
+    for (unsigned i = 0; i < turn; i += U) {
       Row<T> x[U];
 #pragma unroll
       for (int u = 0; u < U; u++)
         if (skey[i + u] != none)
-          load_row<VW, true>(g + (size_t)spos[i + u] * a.width, first, a.G, a.width, x[u]);
+          load_row<VW>(g + (size_t)spos[i + u] * a.width, first, a.G, a.width, x[u]);
 #pragma unroll
       for (int u = 0; u < U; u++) {
+        if (i + u >= turn) break;
         const unsigned k = skey[i + u];
         if (k != cur) {
           if (cur != none) {
@@ -633,83 +736,102 @@ segment_kernel(const T* g, W* gw, Plan a) {
   }
 }
 
-// Joins the sums that cross pieces.  Most take a few pieces: a thread adds four
-// columns' partial sums in order, 1024 columns to a block.  The long ones (at
-// most pieces / kLong) get a block for each 128 columns: eight groups of 32
-// threads add an eighth of the pieces each, in order, then the eight are added
-// in order.  Which block takes which sum does not matter.
+// Joins the sums that cross pieces, 128 columns at a time.  Most take a few
+// pieces: a warp adds the partial sums in order, four columns to a lane.  The
+// long ones (at most pieces / kLong) get a block: its warps add an eighth of the
+// pieces each, in order, then the eight are added in order.  Which block takes
+// which sum does not matter.
 template <class W>
 __global__ void __launch_bounds__(kThreads)
-join_kernel(W* gw, Plan a, unsigned short_tiles, unsigned long_tiles) {
+join_kernel(W* gw, Plan a) {
   __shared__ float4 eighth[8][32];
   wait_for_previous_kernel();   // the partial sums
-  const unsigned part = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const unsigned longs = (a.pieces / kLong + 1) * long_tiles;
-  const bool is_long = blockIdx.x < longs;
-  const unsigned b = is_long ? blockIdx.x : blockIdx.x - longs;
-  const unsigned tiles = is_long ? long_tiles : short_tiles;
-  const unsigned e = b / tiles;
-  if (e >= a.count[is_long]) return;
-  const uint2 which = (is_long ? a.crossing_long : a.crossing)[e];
-  const unsigned piece = which.x;
-  // the pieces after this one whose first key is still the id (keys are
-  // sorted), 32 looked at together
-  unsigned count = 1;   // partial sums: the first one's tail, then heads
-  for (unsigned q = piece + 1; q < a.pieces; q += 32) {
-    const bool more = q + lane < a.pieces && a.pair[(size_t)(q + lane) * a.piece].x == which.y;
-    const unsigned m = __ballot_sync(0xffffffffu, more);
-    count += __popc(m);
-    if (m != 0xffffffffu) break;
-  }
-  const unsigned each = is_long ? (count + 7) / 8 : count;
-  const unsigned j0 = is_long ? part * each : 0, j1 = min(j0 + each, count);
-  const size_t c = is_long ? (size_t)(b % tiles) * 128 + lane * 4
-                           : (size_t)(b % tiles) * (kThreads * 4) + threadIdx.x * 4;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (c < a.width) {
+  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const size_t tiles = (a.width + 127) / 128;
+  const size_t shorts = a.count[0] * tiles, longs = a.count[1] * tiles;
+  for (size_t unit = blockIdx.x; unit < longs + (shorts + 7) / 8; unit += gridDim.x) {
+    const bool is_long = unit < longs;
+    const size_t u = is_long ? unit : (unit - longs) * 8 + warp;
+    if (!is_long && u >= shorts) break;
+    const uint2 which = (is_long ? a.crossing_long : a.crossing)[u / tiles];
+    const unsigned piece = which.x;
+    // the pieces after this one whose first key is still the id (keys are
+    // sorted), 32 looked at together
+    unsigned count = 1;   // partial sums: the first one's tail, then heads
+    for (unsigned q = piece + 1; q < a.pieces; q += 32) {
+      const bool more = q + lane < a.pieces && a.pair[(size_t)(q + lane) * a.piece].x == which.y;
+      const unsigned m = __ballot_sync(0xffffffffu, more);
+      count += __popc(m);
+      if (m != 0xffffffffu) break;
+    }
+    const unsigned each = is_long ? (count + 7) / 8 : count;
+    const unsigned j0 = is_long ? warp * each : 0, j1 = min(j0 + each, count);
+    const size_t c = u % tiles * 128 + lane * 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < a.width) {
 #pragma unroll 8
-    for (unsigned j = j0; j < j1; j++) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(
-          a.partial + (size_t)(piece + j) * 2 * a.ld + (j == 0 ? a.ld : 0) + c));
-      acc.x = fadd(acc.x, x.x);
-      acc.y = fadd(acc.y, x.y);
-      acc.z = fadd(acc.z, x.z);
-      acc.w = fadd(acc.w, x.w);
+      for (unsigned j = j0; j < j1; j++) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(
+            a.partial + (size_t)(piece + j) * 2 * a.ld + (j == 0 ? a.ld : 0) + c));
+        acc.x = fadd(acc.x, x.x);
+        acc.y = fadd(acc.y, x.y);
+        acc.z = fadd(acc.z, x.z);
+        acc.w = fadd(acc.w, x.w);
+      }
     }
-  }
-  if (is_long) {
-    eighth[part][lane] = acc;
-    __syncthreads();
-    if (part != 0) return;
+    if (is_long) {
+      eighth[warp][lane] = acc;
+      __syncthreads();
+      if (warp == 0) {
 #pragma unroll
-    for (int k = 1; k < 8; k++) {
-      const float4 x = eighth[k][lane];
-      acc.x = fadd(acc.x, x.x);
-      acc.y = fadd(acc.y, x.y);
-      acc.z = fadd(acc.z, x.z);
-      acc.w = fadd(acc.w, x.w);
+        for (int k = 1; k < 8; k++) {
+          const float4 x = eighth[k][lane];
+          acc.x = fadd(acc.x, x.x);
+          acc.y = fadd(acc.y, x.y);
+          acc.z = fadd(acc.z, x.z);
+          acc.w = fadd(acc.w, x.w);
+        }
+      }
     }
-  }
-  const float v[4] = {acc.x, acc.y, acc.z, acc.w};
-  W* row = gw + (size_t)which.y * a.width;
+    if (!is_long || warp == 0) {
+      const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+      W* row = gw + (size_t)which.y * a.width;
 #pragma unroll
-  for (int k = 0; k < 4; k++)
-    if (c + k < a.width) {
-      const float r = fmul(v[k], a.scale);
-      row[c + k] = from_f32<W>(a.accumulate ? fadd(to_f32(row[c + k]), r) : r);
+      for (int k = 0; k < 4; k++)
+        if (c + k < a.width) {
+          const float r = fmul(v[k], a.scale);
+          row[c + k] = from_f32<W>(a.accumulate ? fadd(to_f32(row[c + k]), r) : r);
+        }
     }
+    if (is_long) __syncthreads();   // `eighth` is free
+  }
 }
 
 size_t up256(size_t b) { return (b + 255) & ~size_t(255); }
 
 struct Layout {
   unsigned piece, pieces;
+  unsigned G, tiles, per_block;
   size_t ld, list, crossing, partial, total;
 };
-Layout layout_of(size_t n, size_t width) {
+size_t sum_blocks_of(size_t pieces, const Layout& l) {
+  return (pieces * l.tiles + l.per_block - 1) / l.per_block;
+}
+Layout layout_of(StoreType t, size_t n, size_t width) {
   Layout l;
-  size_t piece = kMinPiece;
+  const int N = 16 / (int)store_bytes(t);
+  l.G = group_of(width, N);
+  l.tiles = (unsigned)((width + (size_t)l.G * N - 1) / ((size_t)l.G * N));
+  l.per_block = kThreads / l.G;
+  size_t piece = kPiece;
   while ((n + piece - 1) / piece > kMaxPieces) piece *= 2;
+  // Shorter ones where the blocks would leave SMs idle: a group's positions
+  // come one after the other (1000 ids of 512 bf16, added to a table: 27 us, and
+  // 37 us with 32 positions to a piece).
+  constexpr size_t kBlocks = 2 * 148;
+  while (piece > 1 && sum_blocks_of((n + piece - 1) / piece, l) < kBlocks &&
+         (n + piece / 2 - 1) / (piece / 2) <= kFewPieces)
+    piece /= 2;
   l.piece = (unsigned)piece;
   l.pieces = (unsigned)((n + piece - 1) / piece);
   l.ld = (width + 3) & ~size_t(3);
@@ -723,6 +845,17 @@ Layout layout_of(size_t n, size_t width) {
 cudaError_t sort_ids(IndexArray ids, unsigned n, size_t vocab, long long padding,
                      const Sorted& out, const Shadow& shadow, int* bad, int* passes_out,
                      cudaStream_t s) {
+  int device = 0;
+  cudaGetDevice(&device);
+  const unsigned sms = (unsigned)sm_count(device);
+  if (n <= kFewIds) {
+    *passes_out = 0;
+    const unsigned sorting = (n + kSortWarps - 1) / kSortWarps;
+    const unsigned others = shadow.bytes ? std::max(sms > sorting ? sms - sorting : 0, sms / 2) : 0;
+    few_ids_kernel<<<sorting + others, kSortThreads, 0, s>>>(ids, n, (long long)vocab, padding, out,
+                                                           sorting, shadow, bad);
+    return cudaGetLastError();
+  }
   int total_bits = 1;
   while (total_bits < 32 && (vocab >> total_bits)) total_bits++;
   const int passes = (total_bits + kSortMaxBits - 1) / kSortMaxBits;
@@ -738,12 +871,7 @@ cudaError_t sort_ids(IndexArray ids, unsigned n, size_t vocab, long long padding
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   unsigned others = 0;       // whole clusters, an SM to a block
-  if (shadow.bytes) {
-    int device = 0;
-    cudaGetDevice(&device);
-    const unsigned sms = (unsigned)sm_count(device);
-    others = sms > 2 * blocks ? (sms - blocks) / blocks * blocks : blocks;
-  }
+  if (shadow.bytes) others = sms > 2 * blocks ? (sms - blocks) / blocks * blocks : blocks;
   cfg.gridDim = dim3(blocks + others);
   cfg.blockDim = dim3(kSortThreads);
   cfg.dynamicSmemBytes = smem;
@@ -762,12 +890,10 @@ cudaError_t sort_ids(IndexArray ids, unsigned n, size_t vocab, long long padding
 
 template <class T, class W, int VW>
 cudaError_t sums_of(const void* g, void* gw, Plan a, cudaStream_t s) {
-  constexpr int N = Row<T>::N;
-  a.G = group_of(a.width, N);
-  a.tiles = (unsigned)((a.width + (size_t)a.G * N - 1) / ((size_t)a.G * N));
-  a.per_block = kThreads / a.G;
-  const size_t units = (size_t)a.pieces * a.tiles;
-  const size_t sum_blocks = (units + a.per_block - 1) / a.per_block;
+  int device = 0;
+  cudaGetDevice(&device);
+  const unsigned sms = (unsigned)sm_count(device);
+  const size_t sum_blocks = ((size_t)a.pieces * a.tiles + a.per_block - 1) / a.per_block;
   size_t zero_blocks = 0;
   if (!a.accumulate) {
     // 128 KB of the table to a block that writes zeros
@@ -782,12 +908,10 @@ cudaError_t sums_of(const void* g, void* gw, Plan a, cudaStream_t s) {
                                kThreads, smem, s, static_cast<const T*>(g), static_cast<W*>(gw),
                                a);
   if (e != cudaSuccess || a.pieces < 2) return e;
-  const size_t short_tiles = (a.width + kThreads * 4 - 1) / (kThreads * 4);
-  const size_t long_tiles = (a.width + 127) / 128;
-  const size_t blocks = a.pieces * short_tiles + (a.pieces / kLong + 1) * long_tiles;
-  if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
-  return launch_after(join_kernel<W>, (unsigned)blocks, kThreads, 0, s, static_cast<W*>(gw), a,
-                      (unsigned)short_tiles, (unsigned)long_tiles);
+  const size_t tiles = (a.width + 127) / 128;
+  const size_t blocks = std::min(a.pieces / 8 * tiles + (a.pieces / kLong + 1) * tiles,
+                                 (size_t)16 * sms);
+  return launch_after(join_kernel<W>, (unsigned)blocks, kThreads, 0, s, static_cast<W*>(gw), a);
 }
 
 template <class T, class W>
@@ -816,8 +940,8 @@ cudaError_t launch_embedding(StoreType t, const void* weight, const void* ids, b
   return cudaErrorInvalidValue;
 }
 
-size_t embedding_backward_scratch(size_t n, size_t width) {
-  return layout_of(n, width).total;
+size_t embedding_backward_scratch(StoreType t, size_t n, size_t width) {
+  return layout_of(t, n, width).total;
 }
 
 cudaError_t launch_embedding_backward(StoreType t, const void* grad_output, const void* ids,
@@ -830,7 +954,7 @@ cudaError_t launch_embedding_backward(StoreType t, const void* grad_output, cons
     return accumulate ? cudaSuccess
                       : cudaMemsetAsync(grad_weight, 0,
                                         vocab * width * (narrow ? store_bytes(t) : 4), s);
-  const Layout l = layout_of(n, width);
+  const Layout l = layout_of(t, n, width);
   char* p = static_cast<char*>(scratch);
   Sorted sorted;
   sorted.count = reinterpret_cast<unsigned*>(p);
@@ -857,6 +981,9 @@ cudaError_t launch_embedding_backward(StoreType t, const void* grad_output, cons
   a.n = (unsigned)n;
   a.piece = l.piece;
   a.pieces = l.pieces;
+  a.G = l.G;
+  a.tiles = l.tiles;
+  a.per_block = l.per_block;
   a.pair = sorted.pair[passes & 1];
   a.count = sorted.count;
   a.crossing = reinterpret_cast<uint2*>(p);

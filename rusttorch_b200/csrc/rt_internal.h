@@ -203,7 +203,7 @@ cudaError_t launch_embedding(StoreType t, const void* weight, const void* ids, b
 // grad_weight (f32, or the gradient's type when `narrow`) from grad_output.
 // padding < 0: none.  `scratch`: embedding_backward_scratch bytes, 256-byte
 // aligned.
-size_t embedding_backward_scratch(size_t n, size_t width);
+size_t embedding_backward_scratch(StoreType t, size_t n, size_t width);
 cudaError_t launch_embedding_backward(StoreType t, const void* grad_output, const void* ids,
                                       bool wide, size_t n, size_t vocab, size_t width,
                                       float scale, long long padding, bool accumulate,

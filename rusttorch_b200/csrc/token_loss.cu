@@ -130,8 +130,8 @@ cudaError_t launch_token_loss(const TokenLoss& a, float* loss, float* stats, voi
   const bool here = count && counts_itself(a);
   cudaError_t e = count && !here ? launch_count(a, count, s) : cudaSuccess;
   if (e == cudaSuccess)
-    e = launch_rows(a, none ? loss : sc.row_losses, stats, nullptr, 1.0f, here ? count : nullptr,
-                    here, false, s);
+    e = launch_rows(a, none ? loss : sc.row_losses, stats, nullptr, 1.0f, count, here,
+                    count && !here, s);
   return e != cudaSuccess || none ? e : launch_sum(a, sc, count, loss, s);
 }
 

@@ -495,6 +495,8 @@ row_kernel(const T* logits, LossArgs a, unsigned each) {
     fence_proxy_async_smem();
     fine = __syncthreads_and(fine);
   }
+  // the sum, which waits for this kernel alone, reads the count
+  if (!GRAD && a.count) wait_for_previous_kernel();
   if (!fine) {
     if (threadIdx.x == 0) atomicExch(a.gave_up, 1);
     // what may still be on its way into this block's shared memory
