@@ -4,7 +4,11 @@
 // The tensors' addresses and lengths travel as a kernel argument (at most
 // kMaxTensors of them a launch), so a call copies nothing to the device, keeps
 // nothing, and can be captured.  Every tensor is cut into chunks of kChunk
-// elements, one block each.
+// elements, one block each (f32), or units of kUnit (8 bits).
+//
+// HBM bounds the f32 step (139 M elements in 194 tensors: 605 us, 6.4 TB/s).
+// With 8-bit moments instructions do, before HBM (417 M elements, bf16 gradients
+// and copies: 1.32 ms, 5.1 TB/s).
 #include "rt_adam.cuh"
 #include "rt_internal.h"
 #include "rt_libm.cuh"
@@ -586,7 +590,8 @@ adam8_multi_kernel(const __grid_constant__ Table<CAP> tab, Adam8Coeffs c, unsign
   }
 }
 
-// A warp per block; v arrives as itself and is stored as its root.
+// A warp per block; v arrives as itself and is stored as its root.  (2^27
+// elements: 533 us, and 377 us back: both once in a training run's start.)
 __global__ void __launch_bounds__(kThreads)
 adam8_pack_kernel(const float* m, const float* v, unsigned char* mc, float* ms, unsigned char* vc,
                   float* vs, size_t n) {

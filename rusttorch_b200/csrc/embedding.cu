@@ -527,7 +527,7 @@ few_ids_kernel(IndexArray ids, unsigned n, long long vocab, long long padding, S
 constexpr int kSub = 16;             // sorted positions whose ids are staged at a time
 constexpr int kPiece = 32;           // positions to a piece, unless there are few or very many
 constexpr size_t kMaxPieces = 2048;
-constexpr size_t kFewPieces = 1024;  // at most, where pieces are cut shorter than kPiece
+constexpr size_t kFewPieces = 2048;  // at most, where pieces are cut shorter than kPiece
 constexpr unsigned kLong = 16;       // a sum over more pieces than this is a long one
 constexpr int kZeroRows = 64;        // at most, to a block that writes zeros
 constexpr int kZeroBytes = 4096;     // zeros that it copies at a time

@@ -116,8 +116,8 @@ cudaError_t launch_sum(const TokenLoss& a, const Scratch& sc, const Count* count
 // Few rows are counted by the blocks that work on them, 32 to a thread at
 // most: a kernel less, 2 us of the 12 that 32 rows of 1000 took.  For more rows
 // a kernel of one block counts while the first rows arrive.
-bool counts_itself(const TokenLoss& a) {
-  return fits_cluster(a) && a.rows <= (size_t)32 * row_threads(a);
+bool counts_itself(const TokenLoss& a, const void* grad) {
+  return !walks_rows(a, grad) && a.rows <= (size_t)32 * row_threads(a);
 }
 
 }  // namespace
@@ -127,7 +127,7 @@ cudaError_t launch_token_loss(const TokenLoss& a, float* loss, float* stats, voi
   const Scratch sc = scratch_of(a, scratch);
   const bool none = a.reduction == RTC_REDUCE_NONE;
   Count* count = a.reduction == RTC_REDUCE_MEAN && a.rows ? sc.count : nullptr;
-  const bool here = count && counts_itself(a);
+  const bool here = count && counts_itself(a, nullptr);
   cudaError_t e = count && !here ? launch_count(a, count, s) : cudaSuccess;
   if (e == cudaSuccess)
     e = launch_rows(a, none ? loss : sc.row_losses, stats, nullptr, 1.0f, count, here,
@@ -152,12 +152,12 @@ cudaError_t launch_token_loss_grad(const TokenLoss& a, float grad_scale, float* 
   const bool none = a.reduction == RTC_REDUCE_NONE;
   Count* count = a.reduction == RTC_REDUCE_MEAN && a.rows ? sc.count : nullptr;
   const bool one_pass = fits_cluster(a);
-  const bool here = count && counts_itself(a);
+  const bool here = count && counts_itself(a, grad);
   const bool ahead = count && !here;
   cudaError_t e = ahead ? launch_count(a, count, s) : cudaSuccess;
   if (e == cudaSuccess)
     e = launch_rows(a, none ? loss : sc.row_losses, one_pass ? nullptr : sc.stats,
-                    one_pass ? grad : nullptr, grad_scale, count, here, ahead && one_pass, s);
+                    one_pass ? grad : nullptr, grad_scale, count, here, ahead, s);
   if (e == cudaSuccess && !one_pass)
     e = grad_any(a, sc.stats, nullptr, grad_scale, count, false, grad, false, s);
   return e != cudaSuccess || none ? e : launch_sum(a, sc, count, loss, s);

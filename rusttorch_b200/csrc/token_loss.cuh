@@ -9,11 +9,13 @@
 // of its small loss and gradient, which 1 - p_t would lose.
 //
 // HBM bounds it: the gradient call has to read and write each logit once.  So
-// a row stays in shared memory between its statistics and its gradient, over a
+// there a row stays in shared memory between its statistics and its gradient, over a
 // block or a cluster of up to eight, and while the blocks work on one row the
 // next one's bytes arrive by bulk copy.  What comes next are the two
 // exponentials an element (the SM's special function units give 16 a clock),
-// and about eight other instructions, most of them on pairs.
+// and about eight other instructions, most of them on pairs.  Measured: 4096 x
+// 32768 f32 168 us (6.4 TB/s); 8192 x 50257 bf16 313 us (5.3), where the
+// exponentials take 183 us of every SM and without them it would be 264 us.
 #pragma once
 #include "../../include/rusttorch_cuda.h"
 #include "rt_chain.cuh"
@@ -506,13 +508,13 @@ row_kernel(const T* logits, LossArgs a, unsigned each) {
   }
 }
 
-// Rows that no cluster holds: a block walks the row with a running maximum and
-// sum, in steps of NV vectors a thread.
-constexpr int kLongThreads = 512;
-template <class T>
-__global__ void __launch_bounds__(kLongThreads) long_row_kernel(const T* logits, LossArgs a) {
+// Statistics alone: a block of TH walks a row with a running maximum and sum, in
+// steps of NV vectors a thread.  (8192 x 50257 bf16: 143 us, 5.7 TB/s; 1024 x
+// 600000 f32: 426 us, 5.8 TB/s; 8192 x 50257 with 512 threads: 166 us.)
+template <class T, int TH>
+__global__ void __launch_bounds__(TH) walk_kernel(const T* logits, LossArgs a) {
   constexpr int N = Vec<T>::N;
-  constexpr int kWarps = kLongThreads / 32;
+  constexpr int kWarps = TH / 32;
   constexpr int NV = 4;
   __shared__ float2 pairs[kWarps];
   let_next_kernel_start();
@@ -527,17 +529,17 @@ __global__ void __launch_bounds__(kLongThreads) long_row_kernel(const T* logits,
   const float xt = tg.t >= 0 ? to_f32(x[tg.t]) : 0.0f;
   float m = xe;
   float s = has_edge && (long long)edge != tg.t ? exp_below(xe, against(xe)) : 0.0f;
-  for (unsigned i0 = 0; i0 < sp.vecs; i0 += NV * kLongThreads) {
+  for (unsigned i0 = 0; i0 < sp.vecs; i0 += NV * TH) {
     Vec<T> v[NV];
     Top<T> seen;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-      const unsigned i = i0 + k * kLongThreads + self;
+      const unsigned i = i0 + k * TH + self;
       if (i < sp.vecs) load_vec(x + sp.head + (size_t)i * N, v[k]);
     }
 #pragma unroll
     for (int k = 0; k < NV; k++)
-      if (i0 + k * kLongThreads + self < sp.vecs) seen.see(v[k]);
+      if (i0 + k * TH + self < sp.vecs) seen.see(v[k]);
     const float nm = fmaxf(m, seen.get());
     const Under u = under(against(nm));
     const float shrink = exp_below(m, u.m);
@@ -545,7 +547,7 @@ __global__ void __launch_bounds__(kLongThreads) long_row_kernel(const T* logits,
     m = nm;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-      const unsigned i = i0 + k * kLongThreads + self;
+      const unsigned i = i0 + k * TH + self;
       if (i < sp.vecs) {
         const long long t = tg.t - (long long)sp.head - (long long)i * N;
         if (t >= 0 && t < N) drop(v[k], (int)t);
@@ -561,6 +563,7 @@ __global__ void __launch_bounds__(kLongThreads) long_row_kernel(const T* logits,
   const float ws = warp_sum(fmul(s, exp_below(m, against(wm))));
   if ((self & 31) == 0) pairs[self >> 5] = make_float2(wm, ws);
   __syncthreads();
+  if (a.count) wait_for_previous_kernel();   // the sum, which waits for this kernel alone, reads it
   if (self >= 32) return;
   const float2 p = self < kWarps ? pairs[self] : make_float2(-INFINITY, 0.0f);
   const float top = warp_max(p.x);
@@ -572,8 +575,11 @@ __global__ void __launch_bounds__(kLongThreads) long_row_kernel(const T* logits,
   }
 }
 
-// The gradient from the statistics: `parts` blocks to a row.
-template <class T>
+// The gradient from the statistics: G threads to a row, or `parts` blocks, each
+// thread's loads
+// under way before the statistics arrive.  HBM bounds it (4096 x 32768 f32:
+// 168 us, 6.4 TB/s; 8192 x 50257 bf16: 279 us, 5.9).
+template <class T, unsigned G>
 __global__ void __launch_bounds__(kThreads)
 token_grad_kernel(const T* logits, IndexArray targets, size_t rows, unsigned vocab,
                   long long ignore, const float* stats, const float* upstream, bool per_row,
@@ -581,32 +587,35 @@ token_grad_kernel(const T* logits, IndexArray targets, size_t rows, unsigned voc
                   unsigned parts, bool chained, int* bad) {
   constexpr int N = Vec<T>::N;
   constexpr int U = 4;
-  const size_t row = blockIdx.x / parts;
-  const unsigned part = blockIdx.x % parts;
+  const size_t row0 = (size_t)(blockIdx.x / parts) * (kThreads / G) + threadIdx.x / G;
+  const bool live = G == kThreads || row0 < rows;
+  const size_t row = live ? row0 : rows - 1;     // a thread without a row takes part in the count
+  const unsigned part = blockIdx.x % parts, self = threadIdx.x % G;
   const T* x = logits + row * (size_t)vocab;
   T* g = grad + row * (size_t)vocab;
   const Split sp = split_row(x, vocab);
   const Target tg = target_of(targets[row], vocab, ignore);
-  const unsigned i0 = part * (U * kThreads) + threadIdx.x;
+  const unsigned i0 = part * (U * G) + self;
   Vec<T> v[U];
-  if (tg.counted) {
+  if (live && tg.counted) {
 #pragma unroll
     for (int u = 0; u < U; u++)
-      if (i0 + u * kThreads < sp.vecs) load_vec(x + sp.head + (size_t)(i0 + u * kThreads) * N, v[u]);
+      if (i0 + u * G < sp.vecs) load_vec(x + sp.head + (size_t)(i0 + u * G) * N, v[u]);
   }
   if (chained) wait_for_previous_kernel();
   const float top = stats[3 * row], sum = stats[3 * row + 1], others = stats[3 * row + 2];
   float k = upstream ? upstream[per_row ? row : 0] : grad_scale;
   if (count_here) k = fmul(k, count_rows<kThreads>(targets, rows, ignore).inverse);
   else if (count) k = fmul(k, count->inverse);
+  if (!live) return;
   k = tg.bad ? nan_f() : fmul(k, reciprocal(sum));
-  if (tg.bad && part == 0 && threadIdx.x == 0) atomicExch(bad, 1);
+  if (tg.bad && part == 0 && self == 0) atomicExch(bad, 1);
   const Under ut = under(top);
   const float kf = fmul(k, ut.factor);
   const F2 k2 = f2_of(kf, kf);
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const unsigned i = i0 + u * kThreads;
+    const unsigned i = i0 + u * G;
     if (i < sp.vecs) {
       T* p = g + sp.head + (size_t)i * N;
       Vec<T> r = Vec<T>{{0, 0, 0, 0}};
@@ -619,9 +628,8 @@ token_grad_kernel(const T* logits, IndexArray targets, size_t rows, unsigned voc
       if (t >= 0 && t < N) p[t] = from_f32<T>(fmul(-others, k));
     }
   }
-  if (part == 0 && threadIdx.x < sp.head + sp.tail) {
-    const unsigned j =
-        threadIdx.x < sp.head ? threadIdx.x : sp.vecs * N + threadIdx.x;
+  if (part == 0 && self < sp.head + sp.tail) {
+    const unsigned j = self < sp.head ? self : sp.vecs * N + self;
     g[j] = from_f32<T>(!tg.counted            ? 0.0f
                        : (long long)j == tg.t ? fmul(-others, k)
                                               : fmul(exp_below(to_f32(x[j]), top), k));
@@ -701,25 +709,32 @@ cudaError_t rows_by_size(const TokenLoss& t, const LossArgs& a, bool chained, cu
 }
 
 template <class T>
-cudaError_t long_rows(const TokenLoss& t, const LossArgs& a, cudaStream_t s) {
+cudaError_t walk_rows(const TokenLoss& t, const LossArgs& a, bool chained, cudaStream_t s) {
   if (t.rows > kMaxGrid) return cudaErrorInvalidValue;
-  long_row_kernel<T><<<(unsigned)t.rows, kLongThreads, 0, s>>>(static_cast<const T*>(t.logits), a);
+  const size_t vecs = vecs_of(t);
+  // threads for two steps at least
+  const auto kernel = vecs <= 4096    ? walk_kernel<T, 128>
+                      : vecs <= 16384 ? walk_kernel<T, 256> : walk_kernel<T, 512>;
+  const unsigned threads = vecs <= 4096 ? 128 : vecs <= 16384 ? 256 : 512;
+  const T* x = static_cast<const T*>(t.logits);
+  if (chained) return launch_after(kernel, (unsigned)t.rows, threads, 0, s, x, a);
+  kernel<<<(unsigned)t.rows, threads, 0, s>>>(x, a);
   return cudaGetLastError();
 }
 
 // Statistics and losses of every row, and the gradient unless it is null.
 template <class T>
 cudaError_t rows_any(const TokenLoss& t, const LossArgs& a, bool chained, cudaStream_t s) {
-  if (!fits_cluster(t)) return long_rows<T>(t, a, s);
+  if (walks_rows(t, a.grad)) return walk_rows<T>(t, a, chained, s);
   return a.grad ? rows_by_size<T, true>(t, a, chained, s)
                 : rows_by_size<T, false>(t, a, chained, s);
 }
 
-template <class T>
-cudaError_t grad_of(const TokenLoss& a, const float* stats, const float* upstream,
+template <class T, unsigned G>
+cudaError_t grad_by(const TokenLoss& a, const float* stats, const float* upstream,
                     float grad_scale, const Count* count, bool count_here, void* grad,
                     bool chained, cudaStream_t s) {
-  const size_t parts = std::max<size_t>(1, (vecs_of(a) + 4 * kThreads - 1) / (4 * kThreads));
+  const size_t parts = std::max<size_t>(1, (vecs_of(a) + 4 * G - 1) / (4 * G));
   const size_t step = std::max<size_t>(1, kMaxGrid / parts);
   const bool alike =
       ((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(a.logits)) & 15) == 0;
@@ -732,14 +747,14 @@ cudaError_t grad_of(const TokenLoss& a, const float* stats, const float* upstrea
     const T* x = static_cast<const T*>(a.logits) + off;
     T* g = static_cast<T*>(grad) + off;
     const float* up = upstream && per_row ? upstream + r0 : upstream;
-    const unsigned grid = (unsigned)(rows * parts);
+    const unsigned grid = (unsigned)((rows + kThreads / G - 1) / (kThreads / G) * parts);
     cudaError_t e;
     if (chained && r0 == 0) {
-      e = launch_after(token_grad_kernel<T>, grid, kThreads, 0, s, x, targets, rows,
+      e = launch_after(token_grad_kernel<T, G>, grid, kThreads, 0, s, x, targets, rows,
                        (unsigned)a.vocab, a.ignore, stats, up, per_row, grad_scale, count,
                        count_here, g, alike, (unsigned)parts, true, a.bad);
     } else {
-      token_grad_kernel<T><<<grid, kThreads, 0, s>>>(
+      token_grad_kernel<T, G><<<grid, kThreads, 0, s>>>(
           x, targets, rows, (unsigned)a.vocab, a.ignore, stats + 3 * r0, up, per_row, grad_scale,
           count, count_here, g, alike, (unsigned)parts, false, a.bad);
       e = cudaGetLastError();
@@ -747,6 +762,19 @@ cudaError_t grad_of(const TokenLoss& a, const float* stats, const float* upstrea
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
+}
+
+// Four vectors a thread; a warp at least to a row (16384 x 200 f32: 14 us, and
+// 39 us with a block to each).
+template <class T>
+cudaError_t grad_of(const TokenLoss& a, const float* stats, const float* upstream,
+                    float grad_scale, const Count* count, bool count_here, void* grad,
+                    bool chained, cudaStream_t s) {
+  const size_t vecs = vecs_of(a);
+  const auto by = vecs <= 128   ? grad_by<T, 32>
+                  : vecs <= 256 ? grad_by<T, 64>
+                  : vecs <= 512 ? grad_by<T, 128> : grad_by<T, kThreads>;
+  return by(a, stats, upstream, grad_scale, count, count_here, grad, chained, s);
 }
 
 }  // namespace

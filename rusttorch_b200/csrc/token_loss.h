@@ -56,6 +56,15 @@ inline bool fits_cluster(const TokenLoss& a) {
   return vecs_of(a) <= kMaxCluster * run_vecs(1);
 }
 
+// Whether a block walks a row (walk_kernel) where clusters would hold it: for
+// statistics alone, with rows enough for all SMs, since nothing then has to stay
+// on chip (8192 x 50257 bf16: 143 us for 201, 4096 x 32768 f32: 92 for 117), but
+// not for rows that a warp holds (16384 x 1000 f32: 35 us for 23).
+constexpr size_t kWalkRows = 296;
+inline bool walks_rows(const TokenLoss& a, const void* grad) {
+  return !fits_cluster(a) || (!grad && a.rows >= kWalkRows && vecs_of(a) > run_vecs(16));
+}
+
 // Threads of the blocks that take such rows (rows_by_size).
 inline int row_threads(const TokenLoss& a) {
   const size_t vecs = vecs_of(a);
