@@ -249,7 +249,8 @@ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
   x = mix32_high(x);
   return x ^ (x >> 16);
 }
-// The low half of splitmix64's element i: a tensor's key.
+// Element i of Steele, Lea and Flood's splittable generator (2014), its low
+// half: a tensor's key.
 __device__ __forceinline__ uint32_t tensor_key(unsigned long long seed, unsigned long long i) {
   unsigned long long z = seed + (i + 1) * 0x9E3779B97F4A7C15ull;
   z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;

@@ -84,9 +84,11 @@ def logits_of(n, v, seed, dtype, masked=True):
 
 
 # the longest path of additions that a kernel may take over a row: a thread's own
-# elements one after the other, then 10 halvings of a block and 4 of a cluster
+# elements one after the other in two sums (128 threads at least to a row, or 32
+# to one of 400 vectors, 3200 elements, at most), then 10 halvings of a block and
+# 4 of a cluster
 def chain(v):
-    return v // 128 + 16
+    return v // (64 if v <= 3200 else 128) + 16
 
 
 SHAPES = [(1, 1), (1, 2), (2, 3), (3, 7), (5, 8), (4, 31), (9, 129), (5, 1000), (33, 1024), (300, 257), (6, 4097), (4, 32768), (3, 50257),
@@ -236,6 +238,68 @@ def test_loss_of_ignored_and_bad_targets(rt, v):
         flagged()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [4099, 20001, 70001])
+def test_loss_of_many_rows_of_all_kinds(rt, v, dtype):
+    """Rows for all SMs, extreme ones, ignored ones and bad targets among them."""
+    n = 310
+    x, t = logits_of(n, v, 3, dtype)
+    big = {"float32": 3.4e38, "bfloat16": 3.38e38, "float16": 65504.0}[dtype]
+    x[2] = -big
+    x[12] = -np.inf
+    x[22, v - 1] = np.nan
+    x[32, 0] = np.inf
+    x[42] = -np.inf
+    x[42, t[42]] = 2.0
+    x[52, :] = -big
+    x[52, v // 2] = big / 4
+    x[62] *= 2.0 ** 20 if dtype != "float16" else 64
+    t[72] = v
+    t[82] = -1
+    t[2:53:10] = [5, 6, 7, 8, v // 3, v // 2]
+    x[42] = -np.inf
+    x[42, t[42]] = 2.0
+    t[309], t[308] = v - 1, 0
+    x = K.rounded(x, dtype)
+    want, wg = K.token_loss(x, t, reduction="none")
+    lb, gb = K.token_loss_bounds(x, t, -100, "none", 1.0, chain(v), dtype)
+    X, T = put(rt, x, dtype), rt.Tensor.from_numpy(t)
+    loss, stats = rt.softmax_cross_entropy(X, T, reduction="none")
+    near(loss.to_numpy(), want, lb)
+    flagged()
+    up = rt.Tensor.from_numpy(np.ones(n, np.float32))
+    near(get(rt.softmax_cross_entropy_backward(up, X, T, stats, reduction="none")), wg, gb)
+    flagged()
+    shift, _ = shifted(rt, x, dtype, 1)
+    loss, _ = rt.softmax_cross_entropy(shift, T, reduction="none")
+    near(loss.to_numpy(), want, lb)
+    flagged()
+    # the mean over those that give a number
+    t[~np.isfinite(want)] = -100
+    T = rt.Tensor.from_numpy(t)
+    want, wg = K.token_loss(x, t)
+    lb, gb = K.token_loss_bounds(x, t, -100, "mean", 1.0, chain(v), dtype)
+    loss, stats = rt.softmax_cross_entropy(X, T)
+    near(loss.to_numpy(), want, lb)
+    near(get(rt.softmax_cross_entropy_backward(rt.Tensor.from_numpy(np.float32([1])), X, T, stats)), wg, gb)
+    loss, _ = rt.softmax_cross_entropy_grad(X, T, grad=X)
+    near(loss.to_numpy(), want, lb)
+    near(get(X), wg, gb)
+    no_flag()
+
+
+@pytest.mark.parametrize("v", [3, 100, 511, 1023, 2047])
+def test_loss_gradient_of_many_short_rows(rt, v):
+    n = 1003
+    x, t = logits_of(n, v, v, "float32")
+    want, wg = K.token_loss(x, t)
+    lb, gb = K.token_loss_bounds(x, t, -100, "mean", 1.0, chain(v), "float32")
+    X, T = rt.Tensor.from_numpy(x), rt.Tensor.from_numpy(t)
+    loss, stats = rt.softmax_cross_entropy(X, T)
+    near(loss.to_numpy(), want, lb)
+    near(rt.softmax_cross_entropy_backward(rt.Tensor.from_numpy(np.float32([1])), X, T, stats).to_numpy(), wg, gb)
+
+
 def test_loss_without_rows(rt):
     X, T = rt.Tensor([0, 5]), rt.Tensor([0], dtype="int64")
     loss, grad = rt.softmax_cross_entropy_grad(X, T)
@@ -315,6 +379,31 @@ def test_embedding(rt, n, d, v, dtype):
     no_flag()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [1, 15, 520, 521, 1003])
+def test_embedding_of_many_ids(rt, d, dtype):
+    """Several rows a thread; every start modulo 16 bytes; bad ids among them."""
+    n, v = 700000 // (d + 100), 37
+    rng = np.random.default_rng(d)
+    w = K.rounded(rng.normal(0, 1, (v, d)), dtype)
+    ids = rng.integers(0, v, n)
+    want = K.embedding(w, ids, 1.5, dtype)
+    O, big = shifted(rt, np.zeros((n, d), np.float32), dtype, 1)
+    for a in range(16 // N.DTYPE_BYTES[O._code]):
+        W, _ = shifted(rt, w, dtype, a)
+        rt.embedding(W, rt.Tensor.from_numpy(ids), scale=1.5, out=O)
+        same(get(O), want)
+    around = get(big)
+    assert (around[:1] == 9).all() and (around[1 + n * d:] == 9).all()
+    no_flag()
+    ids[::11], ids[1::13] = v, -7
+    got = get(rt.embedding(W, rt.Tensor.from_numpy(ids), scale=1.5))
+    bad = (ids < 0) | (ids >= v)
+    assert np.isnan(got[bad]).all()
+    same(got[~bad], want[~bad])
+    flagged()
+
+
 def test_embedding_shapes_and_values(rt):
     w = np.arange(12, dtype=np.float32).reshape(4, 3)
     w[1, 1], w[2, 0] = np.nan, np.inf
@@ -379,6 +468,23 @@ def test_embedding_gradient(rt, n, d, v, dtype):
         rt.embedding_backward(G, I, v, scale=0.5, accumulate=True, out=out)
         first = K.rounded(want, dtype).astype(np.float64)
         near(get(out), 2 * want, 2 * bound + np.abs(want) * half * 4 + np.abs(first) * 2.0 ** -22 + 2 * K.least(dtype))
+    no_flag()
+
+
+@pytest.mark.parametrize("n", [255, 2048, 4095, 4096, 4097, 8193])
+@pytest.mark.parametrize("kind", ["apart", "text", "padded"])
+def test_embedding_gradient_of_as_many_ids(rt, n, kind):
+    """Each way to sort, each length of a piece."""
+    rng = np.random.default_rng(n)
+    v, d = 9000, 20
+    ids = rng.permutation(v)[:n] if kind == "apart" else np.minimum((np.exp(rng.random(n) * np.log(v + 1)) - 1).astype(np.int64), v - 1)
+    if kind == "padded":
+        ids[rng.random(n) < 0.9] = 3
+    g = rng.normal(0, 1, (n, d)).astype(np.float32)
+    for padding in (None, 3):
+        want, bound = K.embedding_grad(g, ids, v, 2.0, padding)
+        G, I = rt.Tensor.from_numpy(g), rt.Tensor.from_numpy(ids)
+        near(rt.embedding_backward(G, I, v, scale=2.0, padding_idx=padding).to_numpy(), want, bound + 2.0 ** -24 * np.abs(want))
     no_flag()
 
 
@@ -826,3 +932,84 @@ def test_first_call_of_a_process_is_captured(op):
     r = subprocess.run([sys.executable, "-c", FIRST, op], cwd=Path(__file__).resolve().parents[1],
                        capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip().endswith("fine"), r.stderr[-2000:]
+
+
+def test_two_threads_at_once(rt):
+    import threading
+    torch = pytest.importorskip("torch")
+    states, plain = [state_for_all(rt, 9), state_for_all(rt, 10)], [state_for_all(rt, 9), state_for_all(rt, 10)]
+    for s in plain:
+        for _ in range(20):
+            run_all(rt, s)
+    N.check(N.lib().rtc_synchronize())
+    errors = []
+
+    def work(s, stream):
+        try:
+            N.check(N.lib().rtc_set_stream(ctypes.c_void_p(stream.cuda_stream)))
+            for _ in range(20):
+                run_all(rt, s)
+            N.check(N.lib().rtc_synchronize())
+        except Exception as e:
+            errors.append(e)
+        finally:
+            N.check(N.lib().rtc_set_stream(None))
+
+    threads = [threading.Thread(target=work, args=(s, torch.cuda.Stream())) for s in states]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for s, w in zip(states, plain):
+        for x, y in zip(results(s), results(w)):
+            assert (x == y).all()
+
+
+def wrap(rt, x, dtype):
+    return rt.Tensor.from_device_ptr(x.data_ptr(), x.shape, owner=x, dtype=dtype)
+
+
+def test_embedding_past_32_bits(rt):
+    """More than 2^32 elements: the last rows, and sums that are whole numbers."""
+    torch = pytest.importorskip("torch")
+    n, d, v = (1 << 20) + 12345, 4096, 300
+    ids = torch.arange(n, device="cuda") * 7 % v
+    w = torch.arange(v, device="cuda").repeat_interleave(d).reshape(v, d).to(torch.bfloat16)
+    out = torch.empty(n, d, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    rt.embedding(wrap(rt, w, "bfloat16"), wrap(rt, ids, "int64"), out=wrap(rt, out, "bfloat16"))
+    no_flag()
+    for rows in (slice(0, 5), slice((1 << 20) - 3, (1 << 20) + 3), slice(n - 5, n)):
+        assert torch.equal(out[rows], w[ids[rows]])
+    out.fill_(1.0)
+    torch.cuda.synchronize()
+    gw = rt.embedding_backward(wrap(rt, out, "bfloat16"), wrap(rt, ids, "int64"), v).to_numpy()
+    no_flag()
+    count = np.bincount(ids.cpu().numpy(), minlength=v)
+    assert (gw == count[:, None]).all()
+
+
+def test_loss_past_32_bits(rt):
+    """Equal logits, more than 2^32 of them: loss log V, gradient 1/V and 1/V - 1."""
+    torch = pytest.importorskip("torch")
+    n, v = 33000, 131072
+    x = torch.zeros(n, v, dtype=torch.bfloat16, device="cuda")
+    t = torch.arange(n, device="cuda") % v
+    loss, stats = torch.empty(n, device="cuda"), torch.empty(n, 3, device="cuda")
+    torch.cuda.synchronize()
+    X, T, L, S = wrap(rt, x, "bfloat16"), wrap(rt, t, "int64"), wrap(rt, loss, "float32"), wrap(rt, stats, "float32")
+    rt.softmax_cross_entropy(X, T, reduction="none", loss=L, stats=S)
+    rt.synchronize()
+    # 17 log 2: the log's error and the rounding, 2^-22 each of it
+    assert float((loss.double() - 17 * np.log(2)).abs().max()) <= 17 * np.log(2) * 2.0 ** -21
+    loss.zero_()
+    torch.cuda.synchronize()
+    rt.softmax_cross_entropy_grad(X, T, reduction="none", loss=L, grad=X)
+    no_flag()
+    assert float((loss.double() - 17 * np.log(2)).abs().max()) <= 17 * np.log(2) * 2.0 ** -21
+    for i in (0, 1, 32767, 32768, n - 1):
+        row = x[i].double()
+        assert float(row[i]) == -1.0                 # 2^-17 - 1 in bfloat16
+        row[i] = 2.0 ** -17
+        assert bool((row == 2.0 ** -17).all())
