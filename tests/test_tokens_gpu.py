@@ -471,20 +471,25 @@ def test_embedding_gradient(rt, n, d, v, dtype):
     no_flag()
 
 
-@pytest.mark.parametrize("n", [255, 2048, 4095, 4096, 4097, 8193])
+@pytest.mark.parametrize("n", [255, 2048, 4095, 4096, 4097, 4609, 8193, 33000, 49151, 49152, 49153])
 @pytest.mark.parametrize("kind", ["apart", "text", "padded"])
 def test_embedding_gradient_of_as_many_ids(rt, n, kind):
     """Each way to sort, each length of a piece."""
     rng = np.random.default_rng(n)
     v, d = 9000, 20
-    ids = rng.permutation(v)[:n] if kind == "apart" else np.minimum((np.exp(rng.random(n) * np.log(v + 1)) - 1).astype(np.int64), v - 1)
+    ids = np.resize(rng.permutation(v), n) if kind == "apart" else np.minimum((np.exp(rng.random(n) * np.log(v + 1)) - 1).astype(np.int64), v - 1)
     if kind == "padded":
         ids[rng.random(n) < 0.9] = 3
     g = rng.normal(0, 1, (n, d)).astype(np.float32)
     for padding in (None, 3):
         want, bound = K.embedding_grad(g, ids, v, 2.0, padding)
         G, I = rt.Tensor.from_numpy(g), rt.Tensor.from_numpy(ids)
-        near(rt.embedding_backward(G, I, v, scale=2.0, padding_idx=padding).to_numpy(), want, bound + 2.0 ** -24 * np.abs(want))
+        got = rt.embedding_backward(G, I, v, scale=2.0, padding_idx=padding)
+        near(got.to_numpy(), want, bound + 2.0 ** -24 * np.abs(want))
+        # added to zeros: the same sums in the same order, however the ids were sorted
+        acc = rt.Tensor.from_numpy(np.zeros((v, d), np.float32))
+        rt.embedding_backward(G, I, v, scale=2.0, padding_idx=padding, accumulate=True, out=acc)
+        assert (acc.to_numpy() == got.to_numpy()).all()
     no_flag()
 
 
