@@ -72,8 +72,8 @@ rtc_result one_device(const rtc_tensor* a, const rtc_tensor* b) {
 }
 
 rtc_result apart(const rtc_tensor* out, const rtc_tensor* in, const char* what) {
-  if (overlap(out, in)) return invalid_argument(what, "must not overlap another tensor of the call");
-  return ok();
+  if (!overlap(out, in)) return ok();
+  return invalid_argument(what, "must not overlap another tensor of the call");
 }
 
 // `out` may be `in` itself, but not another range over the same bytes.
@@ -314,7 +314,9 @@ extern "C" rtc_result rtc_softmax_cross_entropy_grad(const rtc_tensor* logits,
 
 namespace {
 
-std::string of(const char* list, size_t i) { return std::string(list) + "[" + std::to_string(i) + "]"; }
+std::string of(const char* list, size_t i) {
+  return std::string(list) + "[" + std::to_string(i) + "]";
+}
 
 constexpr size_t kMaxListed = size_t(1) << 20;
 
@@ -449,7 +451,7 @@ bool plain_like(const rtc_tensor* t, const rtc_tensor* p) {
          (reinterpret_cast<uintptr_t>(t->data) & (dtype_bytes(t->dtype) - 1)) == 0;
 }
 bool plain_moment(const rtc_tensor* t, const rtc_tensor* p, bool eight) {
-  return t->dtype == (eight ? RTC_F8E4M3 : RTC_F32) && plain_like(t, p);
+  return t->dtype == (eight ? int(RTC_F8E4M3) : int(RTC_F32)) && plain_like(t, p);
 }
 bool plain_grad(const rtc_tensor* t, const rtc_tensor* p) {
   StoreType type;
@@ -489,10 +491,11 @@ extern "C" rtc_result rtc_adamw_update_multi(
     const rtc_tensor* p = &params[i];
     AdamTensor& t = list[i];
     // what is right is not named: the names are built for an error alone
-    const bool plain = plain_f32(p) && plain_moment(&m[i], p, eight) && plain_moment(&v[i], p, eight) &&
-                       plain_grad(&grads[i], p) &&
-                       (!eight || (plain_scales(&m_scales[i], p) && plain_scales(&v_scales[i], p))) &&
-                       (!copies || plain_copy(&copies[i], p)) && p->device == params[0].device;
+    const bool plain =
+        plain_f32(p) && p->device == params[0].device && plain_moment(&m[i], p, eight) &&
+        plain_moment(&v[i], p, eight) && plain_grad(&grads[i], p) &&
+        (!eight || (plain_scales(&m_scales[i], p) && plain_scales(&v_scales[i], p))) &&
+        (!copies || plain_copy(&copies[i], p));
     if (!plain) TRY(check_listed(params, grads, m, v, m_scales, v_scales, copies, i));
     store_type(grads[i].dtype, &t.gtype);
     t.ms = eight ? f(&m_scales[i]) : nullptr;

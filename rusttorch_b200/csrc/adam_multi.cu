@@ -8,7 +8,7 @@
 //
 // HBM bounds the f32 step (139 M elements in 194 tensors: 605 us, 6.4 TB/s).
 // With 8-bit moments instructions do, before HBM (417 M elements, bf16 gradients
-// and copies: 1.32 ms, 5.1 TB/s).
+// and copies: 1.33 ms, 5.1 TB/s).
 #include "rt_adam.cuh"
 #include "rt_internal.h"
 #include "rt_libm.cuh"
@@ -348,8 +348,8 @@ struct Stage8 {
 };
 
 // One whole block, four elements to a lane.  At 16 bytes an element the step
-// is bound by instructions (about 75 an element, of them 9 for the IEEE square
-// root and 8 for the random bits) before HBM, so
+// is bound by instructions before HBM (417 M elements in 1.33 ms, about 75 for
+// each, of them 9 for the IEEE square root and 8 for the random bits), so
 // arithmetic that allows it goes in pairs, and where all of a lane's new values
 // are finite and in the format's normal range its rounding asks no question.
 template <class G, int COPY>
@@ -395,7 +395,8 @@ __device__ __forceinline__ void adam8_block(const Stage8& st, const Adam8Coeffs&
   if constexpr (COPY == 1) store_copy4(u.copy, kBF16, o, po);
   if constexpr (COPY == 2) store_copy4(u.copy, kF16, o, po);
   // maxima of sizes (as bits; NaN passed over unless nothing else is there)
-  uint32_t topm = warp_top(f2u(fmaxf(max3(fabsf(nm[0]), fabsf(nm[1]), fabsf(nm[2])), fabsf(nm[3]))));
+  uint32_t topm =
+      warp_top(f2u(fmaxf(max3(fabsf(nm[0]), fabsf(nm[1]), fabsf(nm[2])), fabsf(nm[3]))));
   uint32_t topv = warp_top(f2u(fmaxf(max3(r[0], r[1], r[2]), r[3])));
   const bool odd = topm >= 0x7f800000u || topv >= 0x7f800000u;   // an infinity, or only NaN
   if (odd) {
@@ -552,7 +553,8 @@ adam8_multi_kernel(const __grid_constant__ Table<CAP> tab, Adam8Coeffs c, unsign
         st.unit.key = key;
         // a unit begins at a multiple of its size: the high half of the
         // element's number is the same for all of it
-        st.unit.counter = key + (uint32_t)begin * 0x9E3779B1u + (uint32_t)(begin >> 32) * 0xBB67AE85u;
+        st.unit.counter =
+            key + (uint32_t)begin * 0x9E3779B1u + (uint32_t)(begin >> 32) * 0xBB67AE85u;
       }
       __syncwarp();
       if (lane == 0) {
@@ -587,7 +589,8 @@ adam8_multi_kernel(const __grid_constant__ Table<CAP> tab, Adam8Coeffs c, unsign
   }
   if (!fine) {
     if (lane == 0) atomicExch(gave_up, 1);
-    for (int s = 0; s < kStages; s++, turn++) mbar_wait(&stages[turn % kStages].full, (turn / kStages) & 1);
+    for (int s = 0; s < kStages; s++, turn++)
+      mbar_wait(&stages[turn % kStages].full, (turn / kStages) & 1);
   }
 }
 

@@ -348,7 +348,8 @@ __device__ __forceinline__ void write_shadow(const Shadow& z, uint4* zeros, unsi
 // lane, so key and position travel as one, over all the blocks of a cluster.
 // Ids that have no row (outside the vocabulary, or padding) get key = vocab,
 // which sorts last.
-// The grid's further clusters write zeros (Shadow) meanwhile.
+// The grid's further clusters write zeros (Shadow) meanwhile.  (32768 ids below
+// 131072, two passes: 21 us; 16384 below 50257: 14 us.)
 template <int K, bool HELD>
 __global__ void __launch_bounds__(kSortThreads)
 sort_ids_kernel(IndexArray ids, unsigned n, long long vocab, long long padding, int bits,
@@ -530,7 +531,7 @@ few_ids_kernel(IndexArray ids, unsigned n, long long vocab, long long padding, S
 // it is for sums that are added to what is there: 32768 x 4096 bf16 149 us, and
 // 154 us with sort_ids_kernel; 8000 x 300 f32 27 and 31 us.
 constexpr unsigned kTile = 512, kTiledIds = 96 * kTile, kPerBlock = 256;
-constexpr unsigned kTileStride = kTile + 4;    // words: tiles that are searched together, in other banks
+constexpr unsigned kTileStride = kTile + 4;    // words: tiles searched together, in other banks
 
 // The sum over 4 adjacent lanes.
 __device__ __forceinline__ unsigned sum4(unsigned x) {
@@ -723,7 +724,12 @@ __device__ __forceinline__ void write_zeros(const Plan& a, W* gw) {
   bulk_store_wait();   // `zeros` has been read
 }
 
-// U rows' loads in flight per thread (fewer where a row takes many narrow ones).
+// The sums of pieces of the sorted list, a group of G threads to a piece (and to
+// a tile of the row, where that is longer than a block covers), the rows added in
+// the list's order in f32.  HBM bounds it: each gradient is read once, each row
+// with tokens written (or added to) once, the others zeroed (32768 x 4096 bf16
+// into 131072 rows f32: 119 us for 102 at the copy's rate).  U rows' loads in
+// flight per thread (fewer where a row takes many narrow ones).
 template <class T, class W, int VW>
 __global__ void __launch_bounds__(kThreads)
 segment_kernel(const T* g, W* gw, Plan a) {

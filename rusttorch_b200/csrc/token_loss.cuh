@@ -236,8 +236,8 @@ template <class T>
 __device__ __forceinline__ Split split_row(const T* row, unsigned vocab) {
   constexpr unsigned N = Vec<T>::N;
   Split s;
-  s.head = min((unsigned)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (unsigned)sizeof(T),
-               vocab);
+  const unsigned off = reinterpret_cast<uintptr_t>(row) & 15;
+  s.head = min((16 - off) % 16 / (unsigned)sizeof(T), vocab);
   s.vecs = (vocab - s.head) / N;
   s.tail = vocab - s.head - s.vecs * N;
   return s;
