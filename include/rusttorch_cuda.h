@@ -111,7 +111,10 @@ void* rtc_get_stream(void);
  * then reports RTC_BACKEND_ERROR if a kernel on that GPU gave up one of its
  * bounded waits since the last call (its results are then incomplete), or
  * else RTC_INVALID_ARGUMENT if a token operator met an id or a target outside
- * its vocabulary since then. */
+ * its vocabulary since then.  Both are the GPU's, not a thread's or a
+ * stream's: each is reported once, to whichever thread asks first after it
+ * happened, and with both at hand the first is reported by this call and the
+ * second by the next. */
 rtc_result rtc_synchronize(void);
 /* Failure-path self-test (no reference counterpart): queues a one-thread
  * kernel on the current GPU whose bounded mbarrier wait runs out after 50 ms,

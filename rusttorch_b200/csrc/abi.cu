@@ -57,14 +57,16 @@ extern "C" rtc_result rtc_synchronize(void) {
   if (e != cudaSuccess) return backend_error("cudaStreamSynchronize", e);
   int device = 0;
   cudaGetDevice(&device);
-  const DeviceFlags flags = take_device_flags(device);
-  if (flags.wait_timeout)
-    return fail(RTC_BACKEND_ERROR,
-                "a kernel gave up waiting (for a shared-memory tile or another rank; "
-                "2 s limit); results since the last synchronize are incomplete");
-  if (flags.bad_index)
-    return invalid_argument("ids", "a token id or target was outside the vocabulary since the "
-                                   "last synchronize; the rows it gave are NaN");
+  switch (take_device_flag(device)) {
+    case DeviceFlag::kWaitTimeout:
+      return fail(RTC_BACKEND_ERROR,
+                  "a kernel gave up waiting (for a shared-memory tile or another rank; "
+                  "2 s limit); results since the last synchronize are incomplete");
+    case DeviceFlag::kBadIndex:
+      return invalid_argument("ids", "a token id or target was outside the vocabulary since the "
+                                     "last synchronize; the rows it gave are NaN");
+    case DeviceFlag::kNone: break;
+  }
   return ok();
 }
 

@@ -153,14 +153,10 @@ int* wait_timeout_flag(int device);
 // Host: the flag a kernel sets (to 1) when a token id or target lies outside
 // its vocabulary; as wait_timeout_flag.
 int* bad_index_flag(int device);
-// Host: whether a kernel on `device` gave up a bounded wait, or met an index
-// outside its vocabulary, since the last call (the flags are cleared).
-// Synchronises the device's work first.
-struct DeviceFlags {
-  bool wait_timeout = false;
-  bool bad_index = false;
-};
-DeviceFlags take_device_flags(int device);
+// Host: a flag that a kernel on `device` (the current one) has raised since it
+// was last taken; that one is cleared, the other stays for the next call.
+enum class DeviceFlag { kNone, kWaitTimeout, kBadIndex };
+DeviceFlag take_device_flag(int device);
 // Host: launches a one-thread kernel whose bounded wait runs out (50 ms), to
 // exercise the timeout path: the next rtc_synchronize reports it.
 cudaError_t launch_bounded_wait_probe(int device, cudaStream_t s);

@@ -71,15 +71,35 @@ int* bad_index_flag(int device) {
   return p ? p + 1 : nullptr;
 }
 
-DeviceFlags take_device_flags(int device) {
-  if (!wait_timeout_flag(device)) return {};
+namespace {
+
+// What the last take_flag_kernel took, and the mutex that covers it until it
+// has been read.
+__device__ int g_taken;
+std::mutex g_take_mu;
+
+__global__ void take_flag_kernel(int which) { g_taken = atomicExch(&g_flags[which], 0); }
+
+// Whether flag `which` was up; it is down afterwards.  Read and cleared by one
+// atomic exchange, so that what a kernel on another stream raises meanwhile is
+// either in this answer or still there for the next.
+bool take_flag(int which) {
+  std::lock_guard<std::mutex> lock(g_take_mu);
+  take_flag_kernel<<<1, 1>>>(which);
+  int v = 0;
+  return cudaGetLastError() == cudaSuccess &&
+         cudaMemcpyFromSymbol(&v, g_taken, sizeof v) == cudaSuccess && v != 0;
+}
+
+}  // namespace
+
+DeviceFlag take_device_flag(int device) {
+  if (!wait_timeout_flag(device)) return DeviceFlag::kNone;
   int v[2] = {0, 0};
-  if (cudaMemcpyFromSymbol(v, g_flags, sizeof v) != cudaSuccess) return {};
-  if (v[0] || v[1]) {
-    const int zero[2] = {0, 0};
-    cudaMemcpyToSymbol(g_flags, zero, sizeof zero);
-  }
-  return {v[0] != 0, v[1] != 0};
+  if (cudaMemcpyFromSymbol(v, g_flags, sizeof v) != cudaSuccess) return DeviceFlag::kNone;
+  if (v[0] && take_flag(0)) return DeviceFlag::kWaitTimeout;
+  if (v[1] && take_flag(1)) return DeviceFlag::kBadIndex;
+  return DeviceFlag::kNone;
 }
 
 namespace {

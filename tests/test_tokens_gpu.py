@@ -1018,3 +1018,62 @@ def test_loss_past_32_bits(rt):
         assert float(row[i]) == -1.0                 # 2^-17 - 1 in bfloat16
         row[i] = 2.0 ** -17
         assert bool((row == 2.0 ** -17).all())
+
+
+# ---- reports of bad ids -------------------------------------------------------------------
+
+def reported():
+    """Whether rtc_synchronize reports a bad id."""
+    try:
+        N.check(N.lib().rtc_synchronize())
+        return 0
+    except N.RusttorchError as e:
+        assert e.code == N.INVALID_ARGUMENT and "outside the vocabulary" in str(e)
+        return 1
+
+
+def test_a_bad_id_is_reported_beside_a_wait_that_ran_out(rt):
+    W, I, O = rt.Tensor.from_numpy(np.ones((4, 8), np.float32)), rt.Tensor.from_numpy(np.array([9])), rt.Tensor([1, 8])
+    no_flag()
+    N.check(N.lib().rtc_selftest_bounded_wait())
+    rt.embedding(W, I, out=O)
+    with pytest.raises(N.RusttorchError) as e:
+        N.check(N.lib().rtc_synchronize())
+    assert e.value.code == N.BACKEND_ERROR and "gave up waiting" in str(e.value)
+    flagged()
+
+
+def test_every_bad_id_is_reported_once_while_another_thread_asks(rt):
+    """One thread meets a bad id in each of its rounds and asks at the round's
+    end; another, on a stream of its own, asks all the time.  Whoever asks
+    first gets the report: one for each round, none lost and none twice."""
+    import threading
+    torch = pytest.importorskip("torch")
+    W, I, O = rt.Tensor.from_numpy(np.ones((4, 8), np.float32)), rt.Tensor.from_numpy(np.array([9])), rt.Tensor([1, 8])
+    no_flag()
+    rounds, done, errors, reports = 1000, threading.Event(), [], [0, 0]
+
+    def work(k, stream):
+        try:
+            N.check(N.lib().rtc_set_stream(ctypes.c_void_p(stream.cuda_stream)))
+            if k == 0:
+                for _ in range(rounds):
+                    rt.embedding(W, I, out=O)
+                    reports[0] += reported()
+            else:
+                while not done.is_set():
+                    reports[1] += reported()
+        except BaseException as e:
+            errors.append(e)
+        finally:
+            N.check(N.lib().rtc_set_stream(None))
+            if k == 0:
+                done.set()
+
+    threads = [threading.Thread(target=work, args=(k, torch.cuda.Stream())) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    assert sum(reports) + reported() == rounds, reports
