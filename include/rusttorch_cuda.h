@@ -140,7 +140,8 @@ rtc_result rtc_selftest_ordered_sum(const rtc_tensor* x, int chains, float init,
  *    mish still use a correctly rounded log: within 1 and 6 ulp).
  * Process-wide; the environment variable RTC_MATH_MODE=exact|tolerance sets
  * the initial mode.  Kernels already queued keep the mode they were queued
- * with.  ELU, SELU, the backward ops and the losses are the same in both. */
+ * with.  ELU, SELU, the backward ops, the losses and the token operators are
+ * the same in both. */
 enum { RTC_MATH_TOLERANCE = 0, RTC_MATH_EXACT = 1 };
 rtc_result rtc_set_math_mode(int mode);
 int rtc_get_math_mode(void);
@@ -515,7 +516,11 @@ rtc_result rtc_embedding_backward(const rtc_tensor* grad_output, const rtc_tenso
  * M = max_j x_j and o = the sum of e^(x_j - M) over j != t, a row's loss is
  * log(o + e^(x_t - M)) - (x_t - M), as log1p(o) where x_t = M.  Rows whose
  * target is ignore_index have loss and gradient 0.  RTC_REDUCE_MEAN divides
- * the sum over the other rows by their number (0 if there are none).  `loss`
+ * the sum over the other rows by their number (0 if there are none).  The
+ * exponentials in the gradient of f32 logits are within 2.5 * 2^-23 of e^d for
+ * d = x_j - M rounded to f32, as softmax's are within 1e-6; those in the sums, and
+ * all of 16-bit logits, within (0.62 |d| + 4.6) 2^-23; results below 2^-126
+ * are 0.  `loss`
  * (f32) has one element, or targets' shape with RTC_REDUCE_NONE.  A row whose
  * logits are all -inf, or that holds a NaN or +inf, has loss NaN. */
 enum { RTC_REDUCE_NONE = 0, RTC_REDUCE_MEAN = 1, RTC_REDUCE_SUM = 2 };

@@ -61,27 +61,71 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// 1/x within 2^-23 of itself, x in [1, 2^31] or NaN.
-__device__ __forceinline__ float reciprocal(float x) {
+// The larger, NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 constexpr float kLog2e = 1.44269504f;
+// log 2 as f32, and what that leaves.
+constexpr float kLn2 = 0.693147182f, kLn2Low = -1.90465421e-9f;
+// Below this a term is 0, and it bounds what the split below has to hold.
+constexpr float kLeast = -128.0f;
 
-// e^(x - m), m >= x: the difference, its product with log2 e and the
-// hardware's 2^y (2 ulp) each round once, so the result is within
-// (|x - m| + 2) 2^-23 of itself; results below 2^-126 are 0.
+// e^d for d = x - m <= 0, rounded once as the difference: with y = fl(d log2 e),
+// 2^y times 1 + r, r = d - y log 2 (at most 8e-6, so its square is below 2^-34).
+// The hardware's 2^y is within 2^-22 and the last sum rounds once: within
+// 2.5 * 2^-23 of e^d; results below 2^-126 are 0.
 __device__ __forceinline__ float exp_below(float x, float m) {
-  return exp2_approx(fmul(fsub(x, m), kLog2e));
+  const float d = max_nan(fsub(x, m), kLeast);
+  const float y = fmul(d, kLog2e);
+  const float r = __fmaf_rn(-y, kLn2Low, __fmaf_rn(-y, kLn2, d));
+  const float e = exp2_approx(y);
+  return __fmaf_rn(e, r, e);
+}
+// The two parts of that for a pair: 2^y, not yet multiplied by 1 + r, and r.
+__device__ __forceinline__ void exp_parts2(F2 d, float& ea, float& eb, F2& r) {
+  const F2 y = f2_mul(d, f2_of(kLog2e, kLog2e));
+  r = f2_fma(y, f2_of(-kLn2Low, -kLn2Low), f2_fma(y, f2_of(-kLn2, -kLn2), d));
+  f2_to(y, ea, eb);
+  ea = exp2_approx(ea);
+  eb = exp2_approx(eb);
+}
+__device__ __forceinline__ F2 exp_below2(F2 x, float m) {
+  float a, b;
+  f2_to(f2_sum(x, f2_of(-m, -m)), a, b);
+  F2 r;
+  exp_parts2(f2_of(max_nan(a, kLeast), max_nan(b, kLeast)), a, b, r);
+  return f2_fma(f2_of(a, b), r, f2_of(a, b));
+}
+// The same where a row that holds NaN or +inf is known to be one: the last sum,
+// in [0, 1], saturates, which makes 0 of the NaN that r is far below m and so
+// needs no kLeast; x that is NaN or +inf gives 0 as well.
+__device__ __forceinline__ float fma_sat(float a, float b, float c) {
+  float r;
+  asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ F2 exp_below2_sat(F2 x, float m) {
+  float ea, eb, ra, rb;
+  F2 r;
+  exp_parts2(f2_sum(x, f2_of(-m, -m)), ea, eb, r);
+  f2_to(r, ra, rb);
+  return f2_of(fma_sat(ea, ra, ea), fma_sat(eb, rb, eb));
 }
 
-// e^(x - m) of pairs, m >= x, as 2^(x L - m L) for L = log2 e rounded to f32:
-// m L as `hi`, its f32 value, and the factor 2^lo of what that leaves, so the
-// product x L and the difference round once together, and the result times
-// `factor` is within (|x - m| + 2) 2^-23 of itself.  Where the factor would be
-// far from 1 (`wide`: |m| >= 2^20, or not a number) the difference is taken
-// first, and the factor is 1.
+// What a row's terms are taken under: its maximum m.  For sums, and for the
+// gradient of 16-bit logits (which keeps 12 bits at most), they are 2^(x L - m L)
+// for L = log2 e rounded to f32, with m L as `hi`, its f32 value, and the factor
+// 2^-lo of the `lo` that leaves, by which a sum of terms or the gradient's
+// multiplier is multiplied: one rounding of the exponent (|x - m| 2^-24 of the
+// result), L's own (0.23 of that), the hardware's 2^y twice (2^-22 each), and the
+// product's (2^-24): within (0.62 |x - m| + 4.6) 2^-23 of e^(x - m).  In a sum a
+// term's share e^(x - m) bounds what that gives.  Where lo could be larger (`wide`:
+// |m| >= 2^20, or not a number) they are exp_below2's, and the factor is 1.  The
+// gradient of f32 logits has exp_below2_sat's always, since there the error of
+// an unlikely class would show (3.7e-6 at 80 below the maximum).
 struct Under {
   float m, factor;
   F2 hi;
@@ -99,12 +143,13 @@ __device__ __forceinline__ Under under(float m) {
 }
 template <bool WIDE>
 __device__ __forceinline__ F2 term2(F2 x, const Under& u) {
-  F2 y;
-  if constexpr (WIDE) y = f2_mul(f2_sum(x, f2_of(-u.m, -u.m)), f2_of(kLog2e, kLog2e));
-  else y = f2_fma(x, f2_of(kLog2e, kLog2e), u.hi);
-  float a, b;
-  f2_to(y, a, b);
-  return f2_of(exp2_approx(a), exp2_approx(b));
+  if constexpr (WIDE) {
+    return exp_below2(x, u.m);
+  } else {
+    float a, b;
+    f2_to(f2_fma(x, f2_of(kLog2e, kLog2e), u.hi), a, b);
+    return f2_of(exp2_approx(a), exp2_approx(b));
+  }
 }
 
 // ---- 16 bytes of a row ----------------------------------------------------------
@@ -194,13 +239,24 @@ __device__ __forceinline__ void add_terms(const Vec<T>& v, const Under& u, F2& s
 #pragma unroll
   for (int i = 0; i < Vec<T>::N / 2; i++) s = f2_sum(s, term2<WIDE>(pair_of(v, i), u));
 }
-// v's terms times k (which holds the factor).
+// v's terms times k (grad_factor), of a row whose k is NaN if it holds NaN or +inf.
 template <bool WIDE, class T>
 __device__ __forceinline__ Vec<T> scaled_terms(const Vec<T>& v, const Under& u, F2 k) {
   Vec<T> r;
 #pragma unroll
-  for (int i = 0; i < Vec<T>::N / 2; i++) set_pair(r, i, f2_mul(term2<WIDE>(pair_of(v, i), u), k));
+  for (int i = 0; i < Vec<T>::N / 2; i++) {
+    F2 e;
+    if constexpr (sizeof(T) == 4) e = exp_below2_sat(pair_of(v, i), u.m);
+    else e = term2<WIDE>(pair_of(v, i), u);
+    set_pair(r, i, f2_mul(e, k));
+  }
   return r;
+}
+// k with the factor that scaled_terms leaves out, in both halves.
+template <class T>
+__device__ __forceinline__ F2 grad_factor(float k, const Under& u) {
+  if (sizeof(T) != 4) k = fmul(k, u.factor);
+  return f2_of(k, k);
 }
 
 // Volatile, so that the compiler keeps the registers instead of loading twice.
@@ -467,13 +523,12 @@ row_kernel(const T* logits, LossArgs a, unsigned each) {
     if (rank == 0 && threadIdx.x == 0) finish_row(a, tg, row, top, sum, others, xt);
     if constexpr (GRAD) {
       scale_by_count();
-      // the quotient's roundings (of the hardware's reciprocal and of the
-      // products) are common to the row
-      const float k = tg.bad ? nan_f() : fmul(scale, reciprocal(sum));
+      // the quotient's roundings (of 1/sum and of the products) are common to
+      // the row
+      const float k = tg.bad ? nan_f() : fmul(scale, rcp_rn(sum));
       const Under ut = under(top);
-      const float kf = fmul(k, ut.factor);
-      const F2 k2 = f2_of(kf, kf);
-      if (a.alike && !ut.wide && tg.counted) {
+      const F2 k2 = grad_factor<T>(k, ut);
+      if (a.alike && (sizeof(T) == 4 || !ut.wide) && tg.counted) {
 #pragma unroll 2
         for (unsigned i = threadIdx.x; i < count; i += TH)
           store_vec(gv + (size_t)i * N, scaled_terms<false>(run[i], ut, k2));
@@ -608,11 +663,10 @@ token_grad_kernel(const T* logits, IndexArray targets, size_t rows, unsigned voc
   if (count_here) k = fmul(k, count_rows<kThreads>(targets, rows, ignore).inverse);
   else if (count) k = fmul(k, count->inverse);
   if (!live) return;
-  k = tg.bad ? nan_f() : fmul(k, reciprocal(sum));
+  k = tg.bad ? nan_f() : fmul(k, rcp_rn(sum));
   if (tg.bad && part == 0 && self == 0) atomicExch(bad, 1);
   const Under ut = under(top);
-  const float kf = fmul(k, ut.factor);
-  const F2 k2 = f2_of(kf, kf);
+  const F2 k2 = grad_factor<T>(k, ut);
 #pragma unroll
   for (int u = 0; u < U; u++) {
     const unsigned i = i0 + u * G;

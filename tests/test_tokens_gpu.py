@@ -1077,3 +1077,32 @@ def test_every_bad_id_is_reported_once_while_another_thread_asks(rt):
         t.join()
     assert not errors
     assert sum(reports) + reported() == rounds, reports
+
+
+# ---- how close the loss's terms are -----------------------------------------------------------
+
+@pytest.mark.parametrize("n, v", [(3, 1000), (5, 1003), (700, 260), (3, 50257), (400, 9000), (2, 300001), (2, 600001)])
+def test_f32_loss_gradient_is_as_close_as_softmax(rt, n, v):
+    """Within softmax's 1e-6 for unlikely tokens too: the maximum is 20.5 and every
+    other logit 30 to 86 below it on a grid of 2^-10, so that x_j - M is exact.
+    A gradient is off by its term's 2^y (2^-22) and that one's last sum (2^-24),
+    the product with 1/s and upstream (2^-24 each of the two), 1/s (2^-24), and s,
+    whose largest term, 1, is within 4.6 * 2^-23 and whose others are less than
+    v e^-30 < 2^-24 together, lost or not: less than 19 * 2^-24 in all, of which
+    16 * 2^-24 = 9.6e-7 is allowed.  In
+    the target's, -o/s, what o and s have in common cancels."""
+    rng = np.random.default_rng(v)
+    d = np.round(rng.uniform(30, 86, (n, v)) * 1024) / 1024
+    c, t = rng.integers(0, v, n), rng.integers(0, v, n)
+    t = np.where(t == c, (t + 1) % v, t)
+    d[np.arange(n), c] = 0
+    x = (20.5 - d).astype(np.float32)
+    assert (20.5 - x.astype(np.float64) == d).all()
+    want, wg = K.token_loss(x, t, reduction="none")
+    one, T = rt.Tensor.from_numpy(np.ones(n, np.float32)), rt.Tensor.from_numpy(t)
+    for X in (rt.Tensor.from_numpy(x), shifted(rt, x, "float32", 1)[0]):
+        loss, grad = rt.softmax_cross_entropy_grad(X, T, reduction="none")
+        near(grad.to_numpy(), wg, 16 * 2.0 ** -24 * np.abs(wg))
+        loss, stats = rt.softmax_cross_entropy(X, T, reduction="none")
+        near(rt.softmax_cross_entropy_backward(one, X, T, stats, reduction="none").to_numpy(), wg, 16 * 2.0 ** -24 * np.abs(wg))
+    no_flag()
