@@ -519,7 +519,7 @@ rtc_result rtc_embedding_backward(const rtc_tensor* grad_output, const rtc_tenso
  * the sum over the other rows by their number (0 if there are none).  The
  * exponentials in the gradient of f32 logits are within 2.5 * 2^-23 of e^d for
  * d = x_j - M rounded to f32, as softmax's are within 1e-6; those in the sums, and
- * all of 16-bit logits, within (0.62 |d| + 4.6) 2^-23; results below 2^-126
+ * all of 16-bit logits, within (0.62 |d| + 3.1) 2^-23; results below 2^-126
  * are 0.  `loss`
  * (f32) has one element, or targets' shape with RTC_REDUCE_NONE.  A row whose
  * logits are all -inf, or that holds a NaN or +inf, has loss NaN. */

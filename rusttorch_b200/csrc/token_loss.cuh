@@ -120,8 +120,9 @@ __device__ __forceinline__ F2 exp_below2_sat(F2 x, float m) {
 // for L = log2 e rounded to f32, with m L as `hi`, its f32 value, and the factor
 // 2^-lo of the `lo` that leaves, by which a sum of terms or the gradient's
 // multiplier is multiplied: one rounding of the exponent (|x - m| 2^-24 of the
-// result), L's own (0.23 of that), the hardware's 2^y twice (2^-22 each), and the
-// product's (2^-24): within (0.62 |x - m| + 4.6) 2^-23 of e^(x - m).  In a sum a
+// result), L's own (0.23 of that), the hardware's 2^y (2^-22), the factor's and
+// the product's (2^-24 each; |lo| <= 2^-4, so five terms of its series are
+// within 2^-29): within (0.62 |x - m| + 3.1) 2^-23 of e^(x - m).  In a sum a
 // term's share e^(x - m) bounds what that gives.  Where lo could be larger (`wide`:
 // |m| >= 2^20, or not a number) they are exp_below2's, and the factor is 1.  The
 // gradient of f32 logits has exp_below2_sat's always, since there the error of
@@ -136,8 +137,9 @@ __device__ __forceinline__ Under under(float m) {
   u.m = m;
   u.wide = !(fabsf(m) < 0x1p20f);
   const float hi = fmul(m, kLog2e);
-  const float lo = __fmaf_rn(m, kLog2e, -hi);
-  u.factor = u.wide ? 1.0f : exp2_approx(-lo);
+  const float z = fmul(__fmaf_rn(m, kLog2e, -hi), -kLn2);   // -lo log 2
+  const float tail = __fmaf_rn(__fmaf_rn(__fmaf_rn(z, 1.0f / 24, 1.0f / 6), z, 0.5f), z, 1.0f);
+  u.factor = u.wide ? 1.0f : __fmaf_rn(tail, z, 1.0f);
   u.hi = f2_of(-hi, -hi);
   return u;
 }
