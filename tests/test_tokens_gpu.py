@@ -1127,3 +1127,154 @@ def test_16_bit_loss_terms(rt, dtype):
     near(loss.to_numpy(), want, want * ((0.62 * d + 3.1) * 2.0 ** -23 + 2.0 ** -22))
     loss, _ = rt.softmax_cross_entropy_grad(put(rt, x, dtype), rt.Tensor.from_numpy(a), reduction="none")
     near(loss.to_numpy(), want, want * ((0.62 * d + 3.1) * 2.0 ** -23 + 2.0 ** -22))
+
+
+# ---- more than one turn: buffers in turn, passes of the sort, tables of tensors ---------------
+
+def eight_bit_step(rt, host, gtypes, ctypes_, offsets, hyper, t, seed):
+    """One 8-bit step of `host`'s tensors, every code, scale and copy bit for bit and
+    the parameters within their bound; tensor i starts offsets[i] elements into its buffer."""
+    P, G, M, V, MS, VS, C, codes, keep = [], [], [], [], [], [], [], [], []
+    for h, gtype, ctype, off in zip(host, gtypes, ctypes_, offsets):
+        dev, here = eight(rt, h)
+        for k, (a, kind) in enumerate(((h[0], "float32"), (h[1], gtype))):
+            x, big = shifted(rt, a, kind, off)
+            (P, G)[k].append(x)
+            keep.append(big)
+        M.append(dev[0]), MS.append(dev[1]), V.append(dev[2]), VS.append(dev[3])
+        C.append(rt.Tensor(h[0].shape, dtype=ctype))
+        codes.append(here)
+    rt.adamw_update_multi(P, G, M, V, *hyper, t, m_scales=MS, v_scales=VS, copies=C, seed=seed)
+    for i, h in enumerate(host):
+        want, bound, *after = K.adamw8(h[0].ravel(), h[1].ravel(), *codes[i], *hyper, t, seed, i)
+        got = P[i].to_numpy()
+        near(got.ravel(), want, bound)
+        same(get(C[i]), K.rounded(got, C[i].dtype))
+        for d, w in zip((M[i], MS[i], V[i], VS[i]), after):
+            assert (d.to_numpy().ravel() == w).all(), i
+    for big, off in zip(keep, np.repeat(offsets, 2)):
+        a = get(big)
+        assert (a[:off] == 9).all() and (a[-8:] == 9).all()
+
+
+@pytest.mark.parametrize("wd", [0.0, 0.01])
+def test_adamw_multi_in_8_bits_of_many_units(rt, wd):
+    """5.9 million elements are 2880 units of 2048: six and more to each of the
+    3 * 148 blocks at most that are resident, so that every buffer of a block's three
+    is filled twice and each barrier passes both its phases; whole units and parts of
+    one, tensors that are not aligned, empty ones between, each type of gradient and copy."""
+    rng = np.random.default_rng(40)
+    sizes = [2_200_000, 0, 1_300_001, 2047, 700_003, 128, 900_000, 800_129, 1]
+    host = [adam_state(rng, [n], DTYPES[i % 3]) for i, n in enumerate(sizes)]
+    host[0][2][500_000:500_100] = 0.0
+    host[2][3][::3] *= 1e-9                 # values under the format's normal range
+    eight_bit_step(rt, host, [DTYPES[i % 3] for i in range(9)], [DTYPES[1 + i // 2 % 2] for i in range(9)],
+                   [0, 0, 0, 0, 1, 0, 0, 3, 0], (1e-3, 0.9, 0.999, 1e-8, wd), 7, 3 << 40)
+
+
+@pytest.mark.parametrize("n", [100, 900])
+def test_adamw_multi_in_8_bits_of_very_many_tensors(rt, n):
+    """Lists for the larger arguments of the kernel, and for three launches."""
+    rng = np.random.default_rng(n)
+    host = [adam_state(rng, [int(s)], "bfloat16") for s in rng.integers(0, 400, n)]
+    eight_bit_step(rt, host, ["bfloat16"] * n, ["float16"] * n, [(0, 0, 0, 5)[i % 4] for i in range(n)], HYPER, 3, 77)
+
+
+def test_adamw_multi_in_8_bits_past_32_bits(rt):
+    """A tensor of more than 2^32 elements: its last ones, whose random bits count on."""
+    torch = pytest.importorskip("torch")
+    n, last = (1 << 32) + 70001, 70001 + 300          # whole blocks of 128, and a part, on both sides of 2^32
+    begin = (n - last) // K.BLOCK * K.BLOCK
+    last = n - begin
+    rng = np.random.default_rng(41)
+    tail = rng.normal(0, 1e-2, last).astype(np.float32)
+    p, g = torch.zeros(n, device="cuda"), torch.full((n,), 2.0 ** -7, dtype=torch.bfloat16, device="cuda")
+    tail = K.bf16(tail)
+    g[begin:] = torch.from_numpy(tail).cuda().to(torch.bfloat16)
+    codes, scales = [torch.zeros(n, dtype=torch.uint8, device="cuda") for _ in range(2)], [torch.zeros(-(-n // K.BLOCK), device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    W = lambda x, kind: [wrap(rt, x, kind)]
+    rt.adamw_update_multi(W(p, "float32"), W(g, "bfloat16"), W(codes[0], "float8_e4m3"), W(codes[1], "float8_e4m3"), *HYPER, 1,
+                          m_scales=W(scales[0], "float32"), v_scales=W(scales[1], "float32"), seed=9)
+    no_flag()
+    i = np.arange(begin, n, dtype=np.uint64)
+    with np.errstate(over="ignore"):
+        bits = K.mix32(np.uint32(K.tensor_key(9, 0)) + i.astype(np.uint32) * np.uint32(0x9E3779B1) + (i >> np.uint64(32)).astype(np.uint32) * np.uint32(0xBB67AE85))
+    one = np.float32(1)
+    m = tail * (one - np.float32(0.9))
+    r = np.sqrt((tail * tail) * (one - np.float32(0.999)))
+    for x, least, low, k in ((m, False, bits & np.uint32(0xffff), 0), (r, True, bits >> np.uint32(16), 1)):
+        c, s = K.encode(x, low, least)
+        assert (codes[k][begin:].cpu().numpy() == c).all()
+        assert (scales[k][begin // K.BLOCK:].cpu().numpy() == s).all()
+    # the first ones: all gradients alike, so the first step moves each by lr, to the digits of two quotients
+    assert float((p[:1 << 20] + 1e-3).abs().max()) <= 1e-3 * (2.0 ** -20 + 1e-8 / (2.0 ** -7 * 0.03))
+    del p, g, codes, scales
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n", [5000, 40000, 60001])
+@pytest.mark.parametrize("v, d", [(50257, 3), (131072, 2), (300000, 2), ((1 << 27) + 9, 1)])
+def test_embedding_gradient_of_large_vocabularies(rt, n, v, d):
+    """Two passes of 8 and 9 bits, three and four: whole numbers, so that sums are exact."""
+    rng = np.random.default_rng(n + d)
+    ids = rng.integers(0, v, n)
+    ids[::5] = ids[3]                                 # one that is frequent
+    ids[1::50] = v - 1 - rng.integers(0, 3, len(ids[1::50]))
+    ids[2], ids[n - 1] = 0, v - 1
+    g = rng.integers(-8, 9, (n, d)).astype(np.float32)
+    named, at = np.unique(ids, return_inverse=True)
+    want = np.zeros((len(named), d))
+    np.add.at(want, at, g)
+    G, I = rt.Tensor.from_numpy(g), rt.Tensor.from_numpy(ids)
+    for padding in (None, v - 1):
+        w = np.where((named == padding)[:, None], 0, want) if padding is not None else want
+        out = rt.embedding_backward(G, I, v, padding_idx=padding)
+        got = out.to_numpy()
+        assert (got[named] == w).all()
+        got[named] = 0
+        assert not got.any()
+        # added to it: twice as much
+        rt.embedding_backward(G, I, v, padding_idx=padding, accumulate=True, out=out)
+        got = out.to_numpy()
+        assert (got[named] == 2 * w).all()
+        got[named] = 0
+        assert not got.any()
+    no_flag()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n, v", [(7200, 1000), (3600, 2500), (1800, 5000), (100, 120001)])
+def test_loss_and_gradient_of_several_rows_a_block(rt, n, v, dtype):
+    """Three rows and more to each block (or cluster) that can be resident, for each
+    size of block, ignored rows among them: both buffers, each barrier's phases."""
+    v *= 1 if dtype == "float32" else 2               # the same bytes to a row
+    x, t = logits_of(n, v, n, dtype)
+    rng = np.random.default_rng(n)
+    t[rng.random(n) < 0.3] = -100
+    t[n // 2:n // 2 + n // 10] = -100
+    want, wg = K.token_loss(x, t, reduction="none")
+    lb, gb = K.token_loss_bounds(x, t, -100, "none", 1.0, chain(v), dtype)
+    X, T = put(rt, x, dtype), rt.Tensor.from_numpy(t)
+    loss, grad = rt.softmax_cross_entropy_grad(X, T, reduction="none")
+    near(loss.to_numpy(), want, lb)
+    near(get(grad), wg, gb)
+    loss, grad = rt.softmax_cross_entropy_grad(X, T, reduction="none", grad=X)
+    near(loss.to_numpy(), want, lb)
+    near(get(X), wg, gb)
+    no_flag()
+
+
+def test_a_bigram_model_moves_alike_in_8_bits(rt):
+    """The first step starts from moments of 0, which 8 bits hold exactly: both forms
+    move a parameter alike but for the roundings of their quotients, 16 of 2^-24 in
+    all (8 operations in f32's, and 8 in the other's with 2^-23 for the reciprocal's),
+    and half an ulp of the parameter in each of the two differences on both sides."""
+    table, ids, targets = bigram_data()
+    losses, w, b = bigram(rt, 1, 32, table, ids, targets)
+    losses8, w8, b8 = bigram(rt, 1, 8, table, ids, targets)
+    assert losses == losses8
+    for start, x, y in ((table, w, w8), (np.zeros_like(b), b, b8)):
+        move = np.abs(x.astype(np.float64) - start)
+        assert (move > 0.04).any()
+        near(y, x, 0.05 * 2.0 ** -20 + np.abs(start) * 2.0 ** -22 + np.abs(x) * 2.0 ** -22)
