@@ -21,8 +21,9 @@ MATH_TOLERANCE, MATH_EXACT = 0, 1
 IPC_HANDLE_BYTES, PEER_MAX_RANKS = 64, 8
 # dtype codes and status codes (rusttorch_cuda.h)
 F32, F64, I32, I64, BF16, F16, F8E4M3 = range(7)
-DTYPE_NAMES = {"float32": F32, "float64": F64, "int32": I32, "int64": I64, "bfloat16": BF16,
-               "float16": F16, "float8_e4m3": F8E4M3}
+# what a Tensor may hold
+DTYPE_NAMES = {"float32": F32, "int32": I32, "int64": I64, "bfloat16": BF16, "float16": F16,
+               "float8_e4m3": F8E4M3}
 DTYPE_BYTES = {F32: 4, F64: 8, I32: 4, I64: 8, BF16: 2, F16: 2, F8E4M3: 1}
 # reductions of the token loss (RTC_REDUCE_*)
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}

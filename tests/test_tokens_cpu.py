@@ -255,6 +255,17 @@ def test_python_refusals():
         rt.Tensor.from_numpy(np.zeros(3, np.float32), dtype="float16")
 
 
+def test_no_float64_tensors():
+    """No operator takes them, so none is made: not by name, not from an array."""
+    import rusttorch_b200 as rt
+    with pytest.raises(ValueError, match="dtype must be one of .*not 'float64'"):
+        rt.Tensor([4], ptr=0x1000, dtype="float64")
+    with pytest.raises(ValueError, match="not 'float64'"):
+        rt.Tensor.from_device_ptr(0x1000, [4], dtype="float64")
+    with pytest.raises(rt.RusttorchError):
+        rt.Tensor.from_numpy(np.zeros(3), dtype="float64")
+
+
 # ---- the 8-bit moments' arithmetic --------------------------------------------------
 
 def test_e4m3_table():
