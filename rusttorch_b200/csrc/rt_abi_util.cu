@@ -73,6 +73,9 @@ rtc_result invalid_argument(const std::string& parameter, const std::string& rea
 rtc_result unsupported(const std::string& msg) { return fail(RTC_UNSUPPORTED, msg); }
 
 rtc_result backend_error(const std::string& what, cudaError_t e) {
+  // The runtime keeps the error for cudaGetLastError, which the next call's
+  // launches would take for their own.
+  cudaGetLastError();
   return fail(RTC_BACKEND_ERROR, "CUDA error in " + what + ": " + cudaGetErrorName(e) + " (" +
                                      cudaGetErrorString(e) + ")");
 }

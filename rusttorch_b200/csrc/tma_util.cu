@@ -85,9 +85,9 @@ __global__ void take_flag_kernel(int which) { g_taken = atomicExch(&g_flags[whic
 // either in this answer or still there for the next.
 bool take_flag(int which) {
   std::lock_guard<std::mutex> lock(g_take_mu);
-  take_flag_kernel<<<1, 1>>>(which);
+  void* args[] = {&which};
   int v = 0;
-  return cudaGetLastError() == cudaSuccess &&
+  return cudaLaunchKernel(take_flag_kernel, dim3(1), dim3(1), args, 0, nullptr) == cudaSuccess &&
          cudaMemcpyFromSymbol(&v, g_taken, sizeof v) == cudaSuccess && v != 0;
 }
 

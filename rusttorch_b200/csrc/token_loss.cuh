@@ -74,7 +74,7 @@ constexpr float kLn2 = 0.693147182f, kLn2Low = -1.90465421e-9f;
 constexpr float kLeast = -128.0f;
 
 // e^d for d = x - m <= 0, rounded once as the difference: with y = fl(d log2 e),
-// 2^y times 1 + r, r = d - y log 2 (at most 8e-6, so its square is below 2^-34).
+// 2^y times 1 + r, r = d - y log 2 (at most 7e-6, so its square is below 2^-34).
 // The hardware's 2^y is within 2^-22 and the last sum rounds once: within
 // 2.5 * 2^-23 of e^d; results below 2^-126 are 0.
 __device__ __forceinline__ float exp_below(float x, float m) {

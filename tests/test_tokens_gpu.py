@@ -1278,3 +1278,32 @@ def test_a_bigram_model_moves_alike_in_8_bits(rt):
         move = np.abs(x.astype(np.float64) - start)
         assert (move > 0.04).any()
         near(y, x, 0.05 * 2.0 ** -20 + np.abs(start) * 2.0 ** -22 + np.abs(x) * 2.0 ** -22)
+
+
+# ---- after an error --------------------------------------------------------------------------
+
+def test_a_call_after_one_that_ran_out_of_memory(rt):
+    """An error is reported by the call that met it, and by no later one."""
+    x = rt.Tensor.from_numpy(np.arange(8, dtype=np.float32))
+    W, I, O = rt.Tensor.from_numpy(np.ones((4, 8), np.float32)), rt.Tensor.from_numpy(np.array([9, 1])), rt.Tensor([2, 8])
+    no_flag()
+
+    def fails():
+        with pytest.raises(N.RusttorchError) as e:
+            rt.Tensor([1 << 45])
+        assert e.value.code == N.BACKEND_ERROR and "MemoryAllocation" in str(e.value)
+
+    fails()
+    same(rt.add(x, x).to_numpy(), np.arange(0, 16, 2))
+    fails()
+    rt.embedding(W, I, out=O)
+    fails()
+    flagged()
+    same(O.to_numpy()[1], np.ones(8))
+    G = rt.Tensor.from_numpy(np.ones((2, 8), np.float32))
+    fails()
+    out = rt.Tensor([4, 8])
+    fails()
+    rt.embedding_backward(G, rt.Tensor.from_numpy(np.array([2, 2])), 4, out=out)
+    same(out.to_numpy(), np.repeat([[0], [0], [2], [0]], 8, 1))
+    no_flag()
