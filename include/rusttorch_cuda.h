@@ -507,7 +507,9 @@ rtc_result rtc_embedding(const rtc_tensor* weight, const rtc_tensor* ids, float 
  * depends on ids alone), 0 for a v that no id names; with accumulate != 0 that
  * is added to grad_weight, and rows that no id names are not touched.  Ids
  * equal to padding_idx (negative: none) contribute nothing.  grad_output (ids'
- * shape, D) in T; grad_weight [V, D] in f32 or in T; fewer than 2^31 ids. */
+ * shape, D) in T; grad_weight [V, D] in f32 or in T; fewer than 2^31 ids.  The
+ * call's scratch, from the stream-ordered pool, is 16 bytes an id and at most
+ * 2048 * 2 * D * 4 bytes of partial sums. */
 rtc_result rtc_embedding_backward(const rtc_tensor* grad_output, const rtc_tensor* ids,
                                   float scale, int64_t padding_idx, int accumulate,
                                   const rtc_tensor* grad_weight);
@@ -516,13 +518,13 @@ rtc_result rtc_embedding_backward(const rtc_tensor* grad_output, const rtc_tenso
  * M = max_j x_j and o = the sum of e^(x_j - M) over j != t, a row's loss is
  * log(o + e^(x_t - M)) - (x_t - M), as log1p(o) where x_t = M.  Rows whose
  * target is ignore_index have loss and gradient 0.  RTC_REDUCE_MEAN divides
- * the sum over the other rows by their number (0 if there are none).  The
- * exponentials in the gradient of f32 logits are within 2.5 * 2^-23 of e^d for
- * d = x_j - M rounded to f32, as softmax's are within 1e-6; those in the sums, and
- * all of 16-bit logits, within (0.62 |d| + 3.1) 2^-23; results below 2^-126
- * are 0.  `loss`
+ * the sum over the other rows by their number (0 if there are none).  `loss`
  * (f32) has one element, or targets' shape with RTC_REDUCE_NONE.  A row whose
- * logits are all -inf, or that holds a NaN or +inf, has loss NaN. */
+ * logits are all -inf, or that holds a NaN or +inf, has loss NaN.  The
+ * exponentials in the gradient of f32 logits are within 2.5 * 2^-23 of e^d for
+ * d = x_j - M rounded to f32 (softmax's are within 1e-6); those in the sums, and
+ * all of 16-bit logits, within (0.62 |d| + 3.1) 2^-23.  Exponentials below
+ * 2^-126 are 0. */
 enum { RTC_REDUCE_NONE = 0, RTC_REDUCE_MEAN = 1, RTC_REDUCE_SUM = 2 };
 /* Forward.  `stats` (f32, targets' shape then 3; may be NULL) receives
  * M, o + e^(x_t - M) and o for the backward call. */

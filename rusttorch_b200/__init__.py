@@ -212,7 +212,9 @@ def _bf16_bits(a: np.ndarray) -> np.ndarray:
 class TensorList:
     """Tensors that are passed to a call together, their descriptors laid out
     once: an optimizer keeps one for its parameters, gradients and moments.
-    Wherever a function takes a list of tensors it takes one of these."""
+    Wherever a function takes a list of tensors it takes one of these.  To lay one
+    out takes 0.3 us a tensor, and a Tensor around a pointer 4 us: a program whose
+    gradients are other buffers in each step pays both in each."""
 
     def __init__(self, tensors):
         self.tensors = tuple(tensors)

@@ -8,7 +8,7 @@
 //
 // HBM bounds the f32 step (139 M elements in 194 tensors: 605 us, 6.4 TB/s).
 // With 8-bit moments instructions do, before HBM (417 M elements, bf16 gradients
-// and copies: 1.33 ms, 5.1 TB/s).
+// and copies: 1.34 ms, 5.0 TB/s).
 #include "rt_adam.cuh"
 #include "rt_internal.h"
 #include "rt_libm.cuh"
@@ -268,8 +268,8 @@ __device__ __forceinline__ float warp_max(float x) {
 }
 
 // 1/x within an ulp (x >= 2^-126; 0 from 2^126 on): the step's quotient is
-// within 2 ulp, a 2^-22 part of what a step moves a parameter.  IEEE division
-// took 9 of 87 instructions an element.
+// within 2 ulp, a 2^-22 part of what a step moves a parameter, whose moments
+// have 4 bits.  IEEE division took 9 of 87 instructions an element.
 __device__ __forceinline__ float reciprocal(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -348,8 +348,7 @@ struct Stage8 {
 };
 
 // One whole block, four elements to a lane.  At 16 bytes an element the step
-// is bound by instructions before HBM (417 M elements in 1.33 ms, about 75 for
-// each, of them 9 for the IEEE square root and 8 for the random bits), so
+// is bound by instructions before HBM (417 M elements in 1.34 ms, 72 for each), so
 // arithmetic that allows it goes in pairs, and where all of a lane's new values
 // are finite and in the format's normal range its rounding asks no question.
 template <class G, int COPY>
@@ -595,7 +594,8 @@ adam8_multi_kernel(const __grid_constant__ Table<CAP> tab, Adam8Coeffs c, unsign
 }
 
 // A warp per block; v arrives as itself and is stored as its root.  (2^27
-// elements: 533 us, and 377 us back: both once in a training run's start.)
+// elements: 520 us, and 377 us back, for 209 at the copy's rate: both once in a
+// training run's start.)
 __global__ void __launch_bounds__(kThreads)
 adam8_pack_kernel(const float* m, const float* v, unsigned char* mc, float* ms, unsigned char* vc,
                   float* vs, size_t n) {

@@ -13,8 +13,10 @@
 // block or a cluster of up to eight, and while the blocks work on one row the
 // next one's bytes arrive by bulk copy.  What comes next are the two
 // exponentials an element (the SM's special function units give 16 a clock),
-// and about eight other instructions, most of them on pairs.  Measured: 4096 x
-// 32768 f32 168 us (6.4 TB/s); 8192 x 50257 bf16 313 us (5.3), where the
+// and 12 other instructions (19 for f32, whose gradient's exponentials are
+// closer), most of them on pairs.  Measured: 4096 x 32768 f32 170 us (6.3 TB/s;
+// calls in a row for a tenth of a second draw the GPU's power limit, and a call
+// then takes 181 to 186 us for 176); 8192 x 50257 bf16 316 us (5.2), where the
 // exponentials take 183 us of every SM and without them it would be 264 us.
 #pragma once
 #include "../../include/rusttorch_cuda.h"
@@ -566,8 +568,8 @@ row_kernel(const T* logits, LossArgs a, unsigned each) {
 }
 
 // Statistics alone: a block of TH walks a row with a running maximum and sum, in
-// steps of NV vectors a thread.  (8192 x 50257 bf16: 143 us, 5.7 TB/s; 1024 x
-// 600000 f32: 426 us, 5.8 TB/s; 8192 x 50257 with 512 threads: 166 us.)
+// steps of NV vectors a thread.  (8192 x 50257 bf16: 147 us, 5.6 TB/s; 1024 x
+// 600000 f32: 418 us, 5.9 TB/s; 8192 x 50257 with 512 threads: 166 us.)
 template <class T, int TH>
 __global__ void __launch_bounds__(TH) walk_kernel(const T* logits, LossArgs a) {
   constexpr int N = Vec<T>::N;
@@ -635,7 +637,7 @@ __global__ void __launch_bounds__(TH) walk_kernel(const T* logits, LossArgs a) {
 // The gradient from the statistics: G threads to a row, or `parts` blocks, each
 // thread's loads
 // under way before the statistics arrive.  HBM bounds it (4096 x 32768 f32:
-// 168 us, 6.4 TB/s; 8192 x 50257 bf16: 279 us, 5.9).
+// 170 us, 6.3 TB/s; 8192 x 50257 bf16: 277 us, 6.0).
 template <class T, unsigned G>
 __global__ void __launch_bounds__(kThreads)
 token_grad_kernel(const T* logits, IndexArray targets, size_t rows, unsigned vocab,
@@ -753,7 +755,7 @@ cudaError_t rows_by_size(const TokenLoss& t, const LossArgs& a, bool chained, cu
       // Three blocks to an SM where that puts more rows on it than two do, for
       // 16-bit types (8192 x 32768 bf16: 207 us for 239; at 50257 both put one
       // there, and three take 322 us for 312).  f32, whose time is HBM's, stays
-      // with two (4096 x 32768: 168 us for 177).
+      // with two (4096 x 32768: 178 us for 190 with three, a call).
       const size_t two = (vecs_of(t) + run_vecs(2) - 1) / run_vecs(2);
       const size_t three = (vecs_of(t) + run_vecs(3) - 1) / run_vecs(3);
       if (sizeof(T) == 2 && three <= kMaxCluster && 3 * two > 2 * three)

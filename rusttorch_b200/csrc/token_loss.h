@@ -58,7 +58,7 @@ inline bool fits_cluster(const TokenLoss& a) {
 
 // Whether a block walks a row (walk_kernel) where clusters would hold it: for
 // statistics alone, with rows enough for all SMs, since nothing then has to stay
-// on chip (8192 x 50257 bf16: 143 us for 201, 4096 x 32768 f32: 92 for 117), but
+// on chip (8192 x 50257 bf16: 147 us for 201, 4096 x 32768 f32: 96 for 117), but
 // not for rows that a warp holds (16384 x 1000 f32: 35 us for 23).
 constexpr size_t kWalkRows = 296;
 inline bool walks_rows(const TokenLoss& a, const void* grad) {
