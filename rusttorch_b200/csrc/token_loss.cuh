@@ -14,10 +14,10 @@
 // next one's bytes arrive by bulk copy.  What comes next are the two
 // exponentials an element (the SM's special function units give 16 a clock),
 // and 12 other instructions (19 for f32, whose gradient's exponentials are
-// closer), most of them on pairs.  Measured: 4096 x 32768 f32 170 us (6.3 TB/s;
-// calls in a row for a tenth of a second draw the GPU's power limit, and a call
-// then takes 181 to 186 us for 176); 8192 x 50257 bf16 316 us (5.2), where the
-// exponentials take 183 us of every SM and without them it would be 264 us.
+// closer), most of them on pairs.  Measured: 4096 x 32768 f32 170 us (6.3 TB/s; a
+// call 176 us, on a GPU that a tenth of a second of them brings to its power
+// limit 181 to 186); 8192 x 50257 bf16 316 us (5.2), where the exponentials take
+// 183 us of every SM and without them it would be 264 us.
 #pragma once
 #include "../../include/rusttorch_cuda.h"
 #include "rt_chain.cuh"
